@@ -41,6 +41,7 @@ extern "C" {
 #define BS_ERR_TIMEOUT_PEMPTY 104   /* device status: bounded wait for a TMEM buffer ran out    */
 #define BS_ERR_TIMEOUT_DRAIN 105    /* device status: teardown drain ran out                    */
 #define BS_ERR_TIMEOUT_PEER 106     /* device status: a peer rank did not reach the TP reduce   */
+#define BS_ERR_TIMEOUT_CLUSTER 107  /* device status: a CTA waited too long for one of its cluster */
 #define BS_ERR_TIMEOUT_SELFTEST 199 /* device status: the self-test wait ran out (expected)     */
 
 /* Block-scaled FP8 GEMM:  C[m, n] = sum_kb (A[m, kb] . B[n, kb]) * As[m, kb] * Bs[n/128, kb].
@@ -152,6 +153,59 @@ int bs_fp8_rmsnorm_group_quant(const void* x, int ldx, void* residual, int ldr, 
 /* Tile-first weight pre-pack: tiles[nb][kb][r][c] = W[nb*128 + r][kb*128 + c] for e4m3 W [N, K].
  * Replaces the permute in `relayout(model)` (H:667). W and tiles must not overlap. */
 int bs_fp8_pack_tiles(const void* W, void* tiles, int N, int K, void* stream);
+
+/* ---- mixture of experts (no counterpart in the reference, whose models are dense) ----
+ *
+ * The plan of a routed batch, all int32 on the device: T tokens with top_k slots each, R = T * top_k, e_count local
+ * experts [e_begin, e_begin + e_count) of n_experts.
+ *   offsets   [e_count + 1]  rows of local expert e are offsets[e] .. offsets[e + 1] - 1
+ *   row_token [R]            token of each row; rows sorted by expert, then by t * top_k + s; -1 past offsets[e_count]
+ *   slot_row  [T, top_k]     row of each slot, -1 when its expert is not local (or the slot is empty)
+ *
+ * bs_fp8_moe_route: top-k of the router's logits (dtype 0 = bf16, 1 = fp32; row stride ldl) and the plan.
+ * ids [T, top_k] are the experts with the largest logits in falling order, equal logits by lower index; logits of
+ * -inf or NaN are never chosen, and where fewer than top_k remain the id is -1 and the weight 0. weights [T, top_k]
+ * = scale * softmax over the chosen (renormalize != 0) or over all experts, in fp32. n_experts <= 512, top_k <= 32.
+ * bs_fp8_moe_dispatch: the plan of given ids [T, top_k] (an id outside the local experts has no row).
+ * scratch: bs_fp8_moe_scratch_bytes(T, e_count) bytes, not zeroed, free again when the call's kernels are done
+ * (it may be NULL where that is 0). T == 0 writes zero offsets. */
+int bs_fp8_moe_route(const void* logits, int dtype, long long ldl, int T, int n_experts, int top_k, int renormalize,
+                     float scale, int e_begin, int e_count, float* weights, int* ids, int* offsets, int* row_token,
+                     int* slot_row, void* scratch, size_t scratch_bytes, void* stream);
+int bs_fp8_moe_dispatch(const int* ids, int T, int n_experts, int top_k, int e_begin, int e_count, int* offsets,
+                        int* row_token, int* slot_row, void* scratch, size_t scratch_bytes, void* stream);
+size_t bs_fp8_moe_scratch_bytes(int T, int e_count);
+
+/* Products grouped by expert. Weights: E experts of bs_fp8_gemm's formats one after another (row-major [E, N, K] or
+ * tile-first [E, N/128, K/128, 128, 128]), Bs [E, N/128, K/128]. Row r of the output, offsets[e] <= r < offsets[e + 1],
+ * is row row_token[r] of A (row r where row_token is NULL) times expert e's weights; rows past offsets[E] are
+ * not written. A [rows_a, K], As [rows_a, K/128]; R rows of output. rows_hint: rows that the caller expects
+ * in all (at most R; 0: R); it only chooses between kernels. E <= 512.
+ *   bs_fp8_grouped_gemm             C [R, ldc] bf16 (out_dtype 0) or fp32 (1), as bs_fp8_gemm
+ *   bs_fp8_grouped_gemm_silu_quant  Q [R, I], Qs [R, I/128] with N2 = 2 * I gate and up rows per expert, as
+ *                                   bs_fp8_gemm_silu_quant */
+int bs_fp8_grouped_gemm(const void* A, const void* B, void* C, const float* As, const float* Bs, const int* offsets,
+                        const int* row_token, int rows_a, int R, int rows_hint, int E, int N, int K, int ldc,
+                        int b_tiled, int out_dtype, void* stream);
+int bs_fp8_grouped_gemm_silu_quant(const void* A, const void* B, void* Q, const float* As, const float* Bs, float* Qs,
+                                   const int* offsets, const int* row_token, int rows_a, int R, int rows_hint, int E,
+                                   int N2, int K, int b_tiled, void* stream);
+
+/* The end of a block and the start of the next one, per token t of T, in fp32:
+ *   z = y[t] (bf16, row stride ldy), or with weights and slot_row the sum over s < top_k of weights[t, s] *
+ *       y[slot_row[t, s]] (slots whose row is outside [0, rows_y) add nothing)
+ *   n = z / sqrt(mean(z^2) + eps) * post_weight   (post_weight NULL: n = z)
+ *   h = residual_scale * residual[t] + scale * gate * n
+ *   v = h / sqrt(mean(h^2) + eps) * pre_weight, from the unrounded h; then A, As as bs_fp8_group_quant without a
+ *       rounding of v to bf16 before it   (pre_weight NULL: no A, As)
+ * residual and out are bf16 (wide = 0) or fp32 (1), row strides ldr and ldo; out may be residual. gate_kind 0 none
+ * (1), 1 per channel [H], 2 per token (row stride ldg), 3 per element (row stride ldg); bf16. H: a multiple of
+ * 128, at most 16384; pointers (but a per-token gate's) and row strides in whole 16 bytes. */
+int bs_fp8_block_norm_quant(const void* y, long long ldy, int rows_y, const float* weights, const int* slot_row,
+                            int top_k, const void* residual, long long ldr, void* out, long long ldo, int wide,
+                            const void* post_weight, const void* gate, int gate_kind, long long ldg, float scale,
+                            float residual_scale, const void* pre_weight, float eps, void* A, float* As, int T, int H,
+                            void* stream);
 
 /* Reads the device status word of the current device (synchronises the device). Writes the
  * code to *code and clears it when `clear` is non-zero. Counterpart of the reference's

@@ -1,0 +1,90 @@
+"""CPU: argument checks of the mixture-of-experts entry points (refused before any GPU work) and the oracle's plan."""
+import pytest
+import torch
+
+from oracle import moe as M
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from fp8_hand_b200 import _build, _native
+    _build.build()
+    return _native.lib()
+
+
+P = 1 << 20  # a 16-byte aligned address that is never used: every call below is refused first
+
+
+def test_route_arguments(lib):
+    ok = dict(logits=P, dtype=0, ldl=64, T=4, E=64, k=8, renorm=1, scale=1.0, begin=0, count=64, w=P, ids=P, off=P, rt=P,
+              sr=P, scratch=None, nbytes=0)
+
+    def call(**kw):
+        return lib.bs_fp8_moe_route(*{**ok, **kw}.values(), None)
+
+    for bad in (dict(dtype=2), dict(ldl=63), dict(T=-1), dict(E=513, ldl=600), dict(k=0), dict(k=33), dict(k=9, E=8, count=8),
+                dict(begin=-1), dict(begin=1), dict(count=0), dict(w=None), dict(ids=None), dict(off=None), dict(rt=None),
+                dict(sr=None), dict(logits=None), dict(T=1 << 30)):
+        assert call(**bad) == 1, bad
+    assert call(dtype=1, logits=P + 2) == 2
+
+
+def test_dispatch_arguments(lib):
+    ok = dict(ids=P, T=4, E=64, k=8, begin=0, count=64, off=P, rt=P, sr=P, scratch=None, nbytes=0)
+    for bad in (dict(ids=None), dict(E=0), dict(k=33), dict(begin=60, count=5), dict(off=None), dict(sr=None)):
+        assert lib.bs_fp8_moe_dispatch(*{**ok, **bad}.values(), None) == 1, bad
+
+
+def test_scratch_bytes(lib):
+    assert lib.bs_fp8_moe_scratch_bytes(0, 64) == 0 and lib.bs_fp8_moe_scratch_bytes(1, 64) == 0
+    big = lib.bs_fp8_moe_scratch_bytes(8192, 64)
+    assert big > 0 and big % (64 * 4) == 0
+
+
+def test_grouped_arguments(lib):
+    ok = dict(A=P, B=P, C=P, As=P, Bs=P, off=P, rt=None, rows_a=64, R=64, hint=0, E=8, N=256, K=256, ldc=256, tiled=0, dt=0)
+
+    def call(**kw):
+        return lib.bs_fp8_grouped_gemm(*{**ok, **kw}.values(), None)
+
+    for bad in (dict(K=200), dict(N=200), dict(ldc=128), dict(ldc=260), dict(dt=2), dict(tiled=2), dict(E=0), dict(E=513),
+                dict(rows_a=63), dict(rows_a=0, rt=P), dict(hint=65), dict(R=-1), dict(off=None), dict(A=None), dict(Bs=None),
+                dict(E=512, N=1 << 22, K=128, ldc=1 << 22)):
+        assert call(**bad) == 1, bad
+    assert call(B=P + 8) == 2 and call(C=P + 4) == 2
+    assert call(R=0, rows_a=0, A=None, B=None, C=None, As=None, Bs=None, off=None) == 0
+    fused = dict(A=P, B=P, Q=P, As=P, Bs=P, Qs=P, off=P, rt=P, rows_a=8, R=64, hint=0, E=8, N2=512, K=256, tiled=1)
+    for bad in (dict(N2=384), dict(Qs=None), dict(K=0), dict(tiled=-1)):
+        assert lib.bs_fp8_grouped_gemm_silu_quant(*{**fused, **bad}.values(), None) == 1, bad
+
+
+def test_block_arguments(lib):
+    ok = dict(y=P, ldy=256, rows=4, w=None, sr=None, k=0, res=P, ldr=256, out=P, ldo=256, wide=0, post=None, gate=None, kind=0,
+              ldg=0, scale=1.0, rscale=1.0, pre=P, eps=1e-6, A=P, As=P, T=4, H=256)
+
+    def call(**kw):
+        return lib.bs_fp8_block_norm_quant(*{**ok, **kw}.values(), None)
+
+    for bad in (dict(H=200), dict(H=16512, ldy=16512, ldr=16512, ldo=16512), dict(ldy=128), dict(ldy=260), dict(ldr=258),
+                dict(ldo=250), dict(wide=2), dict(eps=-1.0), dict(eps=float("nan")), dict(kind=1), dict(gate=P), dict(kind=4, gate=P),
+                dict(kind=3, gate=P, ldg=128), dict(kind=2, gate=P, ldg=0), dict(w=P), dict(w=P, sr=P), dict(rows=3), dict(T=-1),
+                dict(A=None), dict(res=None)):
+        assert call(**bad) == 1, bad
+    assert call(y=P + 2) == 2 and call(pre=P + 8) == 2 and call(kind=1, gate=P + 2) == 2
+    assert call(T=0, rows=0) == 0
+
+
+def test_oracle_plan_is_a_stable_sort():
+    ids = torch.tensor([[2, 0], [0, -1], [2, 2], [5, 1]], dtype=torch.int32)
+    off, row_token, slot_row = M.plan(ids, 0, 3)
+    assert off.tolist() == [0, 2, 3, 6]
+    assert row_token.tolist() == [0, 1, 3, 0, 2, 2, -1, -1]
+    assert slot_row.tolist() == [[3, 0], [1, -1], [4, 5], [-1, 2]]
+
+
+def test_host_tensors_are_refused():
+    from fp8_hand_b200 import ops
+    with pytest.raises(ValueError):
+        ops.moe_route(torch.zeros(4, 8), 2)
+    with pytest.raises(ValueError):
+        ops.block_norm_quant(torch.zeros(4, 128, dtype=torch.bfloat16), torch.zeros(4, 128, dtype=torch.bfloat16))

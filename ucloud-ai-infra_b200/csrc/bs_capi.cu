@@ -14,6 +14,9 @@
 #include "bs_decode.cuh"
 #include "bs_quant.cuh"
 #include "bs_tp.cuh"
+#include "bs_route.cuh"
+#include "bs_grouped.cuh"
+#include "bs_block.cuh"
 #include "../../include/bs_fp8.h"
 
 // Library status word: kernels record the first bounded-wait timeout here.
@@ -313,6 +316,38 @@ int max_pair_clusters(int threads, int smem) {
   return st.n[dev];
 }
 
+// Clusters of 2^log_s CTAs of `kern`, one CTA per SM, that fit on the device at once (0 if the query fails).
+template <auto kernel>
+int max_clusters(int threads, int smem, int log_s, int num_sms) {
+  if (log_s == 0) return num_sms;
+  struct State {
+    std::once_flag once[kMaxDevices][4];
+    int n[kMaxDevices][4];
+  };
+  static State st;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices || log_s > 3) return 0;
+  std::call_once(st.once[dev][log_s], [&] {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1u << log_s);
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1u << log_s;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
+    cudaGetLastError();
+    st.n[dev][log_s] = n;
+  });
+  // (num_sms may be capped below the device's SMs)
+  return st.n[dev][log_s] < (num_sms >> log_s) ? st.n[dev][log_s] : num_sms >> log_s;
+}
+
 // Persistent prefill launch. PAIR: clusters of two CTAs on one TPC compute 256-row tiles with
 // cta_group::2 MMAs, one cluster per co-resident SM pair.
 template <bool FUSED, bool PAIR, bool SK = false>
@@ -536,6 +571,8 @@ int launch_row_quant(RowKernel kern, int num_sms, const void* x, int ldx, void* 
                     static_cast<const __nv_bfloat16*>(weight), eps, static_cast<uint8_t*>(A), As, M, K);
 }
 }  // namespace
+
+#include "bs_moe_entry.cuh"
 
 extern "C" {
 
@@ -780,6 +817,7 @@ const char* bs_fp8_error_string(int code) {
     case BS_ERR_TIMEOUT_PFULL: return "device: bounded wait for an MMA partial ran out";
     case BS_ERR_TIMEOUT_PEMPTY: return "device: bounded wait for a TMEM buffer ran out";
     case BS_ERR_TIMEOUT_DRAIN: return "device: teardown drain ran out";
+    case BS_ERR_TIMEOUT_CLUSTER: return "device: bounded wait for a CTA of the same cluster ran out";
     case BS_ERR_TIMEOUT_SELFTEST: return "device: self-test wait ran out (expected)";
     default: return "unknown status code";
   }

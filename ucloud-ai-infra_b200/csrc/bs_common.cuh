@@ -26,6 +26,7 @@ enum : int {
   kErrTimeoutPEmpty = 104,   // MMA issuer waited too long for a free TMEM partial buffer
   kErrTimeoutDrain = 105,    // teardown waited too long for in-flight copies / MMAs
   kErrTimeoutPeer = 106,     // tensor-parallel reduce: a peer rank's CTA did not arrive in time
+  kErrTimeoutCluster = 107,  // a CTA waited too long for another CTA of its cluster
   kErrTimeoutSelftest = 199, // the self-test wait ran out, as it is meant to
 };
 
@@ -87,6 +88,26 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
         *abort = 1;
         return false;
       }
+    }
+  }
+}
+
+// mbar_wait by a whole converged warp: every lane returns the same answer, also when it gives up, so warp-wide
+// instructions may follow.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, int* status,
+                                               int code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const uint64_t t0 = globaltimer_ns();
+  uint32_t spins = 0;
+  while (true) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((spins++ & 63u) == 0) {
+      const bool late = globaltimer_ns() - t0 > kWaitLimitNs;
+      if (late) {
+        atomicCAS(status, 0, code);
+        *abort = 1;
+      }
+      if (__any_sync(0xffffffffu, late || *abort)) return false;
     }
   }
 }

@@ -1,0 +1,862 @@
+// Block-scaled FP8 products grouped by expert, ragged row counts, for sm_100a:
+//     C[r, n] = sum_kb P_kb[r, n] * (As[src(r), kb] * Bs[e, n / 128, kb]),  offsets[e] <= r < offsets[e + 1]
+// P_kb the fp32 product of one 128-wide K block of e4m3 rows and expert e's e4m3 weights, promoted as in
+// bs_prefill.cuh. src(r) = row_token[r] (the rows are read in place, by a gathering TMA load) or r. FUSED: the
+// weights are [gate; up], and the output is Q, Qs of silu(g) * u per 128-column group (bs_prefill.cuh).
+//
+// The row counts are known on the device only: every CTA turns the offsets into a table of the experts that have
+// rows, with the first tile of each, and walks tiles blockIdx.x, blockIdx.x + gridDim.x, ... of the whole list. Tiles
+// of one expert are adjacent, row tiles fastest, so an expert's weights come from HBM once and its row tiles
+// share them in L2.
+//
+// Two kernels. k_grouped_rows: 128 rows x 256 weight columns per tile, rows on the MMA's 128 lanes: tensor bound,
+// for experts with many rows. k_grouped_tokens: 128 weight rows on the lanes, up to NT rows on the columns: bound by
+// the weights' stream, for experts with few rows.
+#pragma once
+#include "bs_common.cuh"
+#include "bs_prefill.cuh"
+#include "bs_route.cuh"
+
+namespace bs {
+
+struct GroupedParams {
+  int E, R;             // local experts; rows of the output
+  int rows_a;           // rows of A
+  int nblk;             // 128-row weight blocks per expert
+  int KB;
+  int ldc;              // plain: row stride of the output, in elements
+  int b_tiled, out_f32;
+  const int* offsets;   // [E + 1]
+  const int* row_token; // [R]: row of A for each row; nullptr: the row itself
+  const float* As;      // [rows_a, KB]
+  const float* Bs;      // [E, nblk, KB]
+  void* out;            // plain: [R, ldc]; fused: Q [R, I]
+  float* qs;            // fused: [R, I / 128]
+  int* status;
+};
+
+// 4 rows x 128 bytes: rows y0..y3 of a map whose box is one row high, 128-byte swizzle.
+__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, uint64_t* bar, int x, const int4& y,
+                                            uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w),
+      "l"(policy)
+      : "memory");
+}
+
+// The experts that have rows, in order.
+struct GroupTable {
+  int n, tiles;
+  int expert[kMaxExperts];
+  int row0[kMaxExperts], rows[kMaxExperts];
+  int tile0[kMaxExperts];  // first tile of the expert
+};
+
+// One warp. An offset outside [0, R] or below its predecessor counts as that bound, so a bad plan reads and writes
+// nothing outside the buffers.
+__device__ __forceinline__ void build_table(GroupTable& g, const GroupedParams& p, int tile_rows, int num_n) {
+  const int lane = threadIdx.x & 31;
+  int n = 0, tiles = 0;
+  for (int e0 = 0; e0 < p.E; e0 += 32) {
+    const int e = e0 + lane;
+    int lo = 0, rows = 0;
+    if (e < p.E) {
+      lo = min(max(__ldcg(p.offsets + e), 0), p.R);
+      rows = max(min(__ldcg(p.offsets + e + 1), p.R) - lo, 0);
+    }
+    const uint32_t has = __ballot_sync(0xffffffffu, rows > 0);
+    const int mine = (rows + tile_rows - 1) / tile_rows * num_n;
+    int inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    if (rows > 0) {
+      const int i = n + __popc(has & ((1u << lane) - 1));
+      g.expert[i] = e;
+      g.row0[i] = lo;
+      g.rows[i] = rows;
+      g.tile0[i] = tiles + inc - mine;
+    }
+    n += __popc(has);
+    tiles += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  if (lane == 0) {
+    g.n = n;
+    g.tiles = tiles;
+  }
+}
+
+struct GroupTile {
+  int expert, tn;
+  int row, rows;  // first row, rows of this tile (1 .. tile_rows)
+};
+
+// Tile -> expert (binary search), weight column tile and row tile.
+__device__ __forceinline__ GroupTile find_tile(const GroupTable& g, int tile, int tile_rows) {
+  int lo = 0, hi = g.n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (g.tile0[mid] <= tile) lo = mid;
+    else hi = mid;
+  }
+  const int in = tile - g.tile0[lo];
+  const int tm = (g.rows[lo] + tile_rows - 1) / tile_rows;
+  GroupTile t;
+  t.expert = g.expert[lo];
+  t.tn = in / tm;
+  const int m = in - t.tn * tm;
+  t.row = g.row0[lo] + m * tile_rows;
+  t.rows = min(g.rows[lo] - m * tile_rows, tile_rows);
+  return t;
+}
+
+// Row of A behind output row r.
+__device__ __forceinline__ int source_row(const GroupedParams& p, int r) {
+  if (!p.row_token) return r < p.rows_a ? r : 0;
+  const int t = __ldg(p.row_token + r);
+  return static_cast<unsigned>(t) < static_cast<unsigned>(p.rows_a) ? t : 0;
+}
+
+// ---------------------------------------------------------------- many rows per expert
+// Roles, stages, TMEM buffers and the promotion are those of k_prefill (bs_prefill.cuh); the producer is a whole warp
+// when the rows are gathered: lane l brings rows 4l..4l+3 of the tile with one gathering load per K block.
+template <bool FUSED>
+struct GroupedRowsCfg {
+  using Regs = RegSplit<384, 168, 40, 232>;
+  static constexpr int kThreads = Regs::kThreads;
+  static constexpr int kStages = 4;
+  static constexpr int kABytes = 128 * 128;
+  static constexpr int kStageBytes = kABytes + 256 * 128;
+  static constexpr int kXchOff = kStages * kStageBytes;
+  static constexpr int kXchBytes = FUSED ? 128 * 2 * 4 : 0;
+  static constexpr int kBarOff = kXchOff + kXchBytes;
+  static constexpr int kTableOff = kBarOff + 256;
+  static constexpr int kSmemBytes = kTableOff + static_cast<int>(sizeof(GroupTable)) + 1024;
+  static constexpr int kTmemCols = 512;
+};
+
+template <bool FUSED>
+__global__ void __launch_bounds__(GroupedRowsCfg<FUSED>::kThreads, 1)
+    k_grouped_rows(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                   const GroupedParams p) {
+  using Cfg = GroupedRowsCfg<FUSED>;
+  constexpr int S = Cfg::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::kBarOff);  // [S] TMA -> MMA
+  uint64_t* empty = full + S;                                         // [S] MMA -> TMA
+  uint64_t* pfull = empty + S;                                        // [2] MMA -> promotion
+  uint64_t* pempty = pfull + 2;                                       // [2] promotion -> MMA
+  uint64_t* drain = pempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* amax_x = reinterpret_cast<float*>(smem + Cfg::kXchOff);  // fused: [128 rows][2 halves]
+  GroupTable& table = *reinterpret_cast<GroupTable*>(smem + Cfg::kTableOff);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&pfull[i], 1);
+      mbar_init(&pempty[i], 256);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    grid_dep_launch();
+  }
+  const int KB = p.KB, nblk = p.nblk;
+  const int I_blk = FUSED ? nblk / 2 : 0;
+  const int num_n = FUSED ? I_blk : (nblk + 1) / 2;
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, Cfg::kTmemCols);
+    tmem_relinquish();
+  }
+  grid_dep_wait();  // the plan, the rows and the output may belong to the previous kernel
+  if (warp == 0) build_table(table, p, 128, num_n);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int num_tiles = table.tiles;
+
+  if (warp >= 8) {
+    regs_decrease<Cfg::Regs::kProducer>();
+    if (warp == 8) {
+      // ------------------------------------------------------------ TMA producer
+      const uint64_t pol_a = policy_evict_last(), pol_b = policy_evict_normal();
+      const bool gather = p.row_token != nullptr;
+      int s = 0;
+      uint32_t ph = 0, issued = 0, parity_bits = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
+        const GroupTile t = find_tile(table, tile, 128);
+        int4 rows = make_int4(0, 0, 0, 0);
+        if (gather) {
+          const int last = t.row + t.rows - 1, r = t.row + 4 * lane;
+          rows = make_int4(source_row(p, min(r, last)), source_row(p, min(r + 1, last)),
+                           source_row(p, min(r + 2, last)), source_row(p, min(r + 3, last)));
+        }
+        const int nb = t.expert * nblk;
+        for (int kb = 0; kb < KB; ++kb) {
+          if (lane == 0) ok = mbar_wait(&empty[s], ph ^ 1, abort_flag, p.status, kErrTimeoutEmpty);
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+          if (!ok) break;
+          uint8_t* st = smem + s * Cfg::kStageBytes;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&full[s], Cfg::kStageBytes);
+            if constexpr (FUSED) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                load_weight_half(st + Cfg::kABytes + 16384 * h, &tmB, &full[s], nb + t.tn, h, kb, KB, p.b_tiled, pol_b);
+                load_weight_half(st + Cfg::kABytes + 16384 * h + 8192, &tmB, &full[s], nb + t.tn + I_blk, h, kb, KB,
+                                 p.b_tiled, pol_b);
+              }
+            } else {
+              load_weight_box(st + Cfg::kABytes, &tmB, &full[s], nb + 2 * t.tn, kb, KB, p.b_tiled, pol_b);
+              load_weight_box(st + Cfg::kABytes + 16384, &tmB, &full[s], nb + 2 * t.tn + 1, kb, KB, p.b_tiled, pol_b);
+            }
+            if (!gather) tma_load_2d(st, &tmA, &full[s], kb * 128, t.row, pol_a);
+          }
+          __syncwarp();
+          if (gather) tma_gather4(st + 512 * lane, &tmA, &full[s], kb * 128, rows, pol_a);
+          issued |= 1u << s;
+          parity_bits = (parity_bits & ~(1u << s)) | (ph << s);
+          if (++s == S) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+      if (!ok && lane == 0)  // leave no copy in flight
+        for (int i = 0; i < S; ++i)
+          if (issued & (1u << i))
+            mbar_wait(&full[i], (parity_bits >> i) & 1u, abort_flag, p.status, kErrTimeoutDrain, 100000000ull);
+    } else if (warp == 9 && lane == 0) {
+      // ------------------------------------------------------------ MMA issuer
+      constexpr uint32_t idesc = idesc_e4m3_f32(128, 256);
+      int s = 0, b = 0;
+      uint32_t ph = 0, pph = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
+        for (int kb = 0; kb < KB; ++kb) {
+          ok = mbar_wait(&full[s], ph, abort_flag, p.status, kErrTimeoutFull) &&
+               mbar_wait(&pempty[b], pph ^ 1, abort_flag, p.status, kErrTimeoutPEmpty);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(smem + s * Cfg::kStageBytes);
+          const uint32_t b0 = a0 + Cfg::kABytes;
+          const uint32_t d = tmem + static_cast<uint32_t>(b * 256);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_e4m3(d, desc_kmajor_sw128(a0 + 32 * k), desc_kmajor_sw128(b0 + 32 * k), idesc, k > 0 ? 1u : 0u);
+          mma_commit(&empty[s]);
+          mma_commit(&pfull[b]);
+          if (++s == S) {
+            s = 0;
+            ph ^= 1;
+          }
+          if (++b == 2) {
+            b = 0;
+            pph ^= 1;
+          }
+        }
+      }
+      mma_commit(drain);
+      mbar_wait(drain, 0, abort_flag, p.status, kErrTimeoutDrain, 100000000ull);
+    }
+  } else {
+    regs_increase<Cfg::Regs::kConsumer>();
+    // ------------------------------------------------------------ promotion + epilogue (as in k_prefill)
+    const int wg = warp >> 2;
+    const int q = warp & 3;
+    const int r = q * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
+    int b = 0;
+    uint32_t pph = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x) {
+      const GroupTile t = find_tile(table, tile, 128);
+      const bool row_ok = r < t.rows;
+      const int row = t.row + (row_ok ? r : 0);
+      const int nb = FUSED ? t.tn : 2 * t.tn + wg;  // block inside the expert; fused: the gate's
+      const bool col_ok = nb < nblk;
+      const float* as_row = p.As + static_cast<size_t>(source_row(p, row)) * KB;
+      const float* bs_row = p.Bs + (static_cast<size_t>(t.expert) * nblk + (col_ok ? nb : 0)) * KB;
+      const float* bu_row = bs_row + static_cast<size_t>(FUSED ? I_blk : 0) * KB;
+
+      uint64_t acc[64];
+#pragma unroll
+      for (int i = 0; i < 64; ++i) acc[i] = 0;
+      auto promote = [&](uint64_t sc2, uint64_t scu2) {
+        if (ok && !mbar_wait_warp(&pfull[b], pph, abort_flag, p.status, kErrTimeoutPFull)) ok = false;
+        if (ok) {
+          tc_fence_after();
+          const uint32_t tbase = tmem + lane_addr + static_cast<uint32_t>(b * 256 + wg * 128);
+          uint32_t v[64];
+          tmem_ld64(tbase, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) ffma2(acc[i], v[2 * i], v[2 * i + 1], sc2);
+          tmem_ld64(tbase + 64, v);
+          tmem_ld_wait();
+          mbar_arrive(&pempty[b]);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) ffma2(acc[32 + i], v[2 * i], v[2 * i + 1], scu2);
+        }
+        if (++b == 2) {
+          b = 0;
+          pph ^= 1;
+        }
+      };
+      if constexpr (FUSED) {
+        constexpr int D = 4;  // scales in groups of four K blocks, one group ahead
+        float sa[D], sg[D], su[D];
+#pragma unroll
+        for (int j = 0; j < D; ++j) {
+          const int k = j < KB ? j : KB - 1;
+          sa[j] = ldg_f32(as_row + k);
+          sg[j] = ldg_f32(bs_row + k);
+          su[j] = ldg_f32(bu_row + k);
+        }
+        for (int kb0 = 0; kb0 < KB; kb0 += D) {
+          float na[D], ng[D], nu[D];
+#pragma unroll
+          for (int j = 0; j < D; ++j) {
+            const int kn = kb0 + D + j < KB ? kb0 + D + j : KB - 1;
+            na[j] = ldg_f32(as_row + kn);
+            ng[j] = ldg_f32(bs_row + kn);
+            nu[j] = ldg_f32(bu_row + kn);
+          }
+#pragma unroll
+          for (int j = 0; j < D; ++j) {
+            if (kb0 + j >= KB) break;
+            const float scg = __fmul_rn(sa[j], sg[j]), scu = __fmul_rn(sa[j], su[j]);
+            promote(pack_f2(scg, scg), pack_f2(scu, scu));
+          }
+#pragma unroll
+          for (int j = 0; j < D; ++j) {
+            sa[j] = na[j];
+            sg[j] = ng[j];
+            su[j] = nu[j];
+          }
+        }
+      } else {
+        const int kn1 = KB > 1 ? 1 : 0;
+        float a_n0 = ldg_f32(as_row), b_n0 = ldg_f32(bs_row);
+        float a_n1 = ldg_f32(as_row + kn1), b_n1 = ldg_f32(bs_row + kn1);
+        for (int kb = 0; kb < KB; ++kb) {
+          const float sa = a_n0, sb = b_n0;
+          a_n0 = a_n1;
+          b_n0 = b_n1;
+          if (kb + 2 < KB) {
+            a_n1 = ldg_f32(as_row + kb + 2);
+            b_n1 = ldg_f32(bs_row + kb + 2);
+          }
+          const float sc = __fmul_rn(sa, sb);
+          promote(pack_f2(sc, sc), pack_f2(sc, sc));
+        }
+      }
+
+      if constexpr (!FUSED) {
+        if (ok && row_ok && col_ok) {
+          const size_t at = static_cast<size_t>(row) * p.ldc + static_cast<size_t>(nb) * 128;
+          if (p.out_f32) {
+            float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              dst[j] = make_float4(lo_f(acc[2 * j]), hi_f(acc[2 * j]), lo_f(acc[2 * j + 1]), hi_f(acc[2 * j + 1]));
+          } else {
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + at);
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              dst[j] = make_uint4(pack_bf16x2(lo_f(acc[4 * j]), hi_f(acc[4 * j])),
+                                  pack_bf16x2(lo_f(acc[4 * j + 1]), hi_f(acc[4 * j + 1])),
+                                  pack_bf16x2(lo_f(acc[4 * j + 2]), hi_f(acc[4 * j + 2])),
+                                  pack_bf16x2(lo_f(acc[4 * j + 3]), hi_f(acc[4 * j + 3])));
+          }
+        }
+      } else {
+        float amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float y0 = silu_mul(lo_f(acc[i]), lo_f(acc[32 + i]));
+          const float y1 = silu_mul(hi_f(acc[i]), hi_f(acc[32 + i]));
+          acc[i] = pack_f2(y0, y1);
+          amax = fmaxf(amax, fmaxf(fabsf(y0), fabsf(y1)));
+        }
+        amax_x[r * 2 + wg] = amax;
+        named_bar_sync(1, 256);
+        amax = fmaxf(amax_x[r * 2], amax_x[r * 2 + 1]);
+        const float scale = __fdiv_rn(fmaxf(amax, 1e-10f), 448.0f);
+        const float inv = __fdiv_rn(1.0f, scale);
+        if (ok && row_ok) {
+          if (wg == 0) p.qs[static_cast<size_t>(row) * I_blk + t.tn] = scale;
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + static_cast<size_t>(row) * I_blk * 128 +
+                                                static_cast<size_t>(t.tn) * 128 + wg * 64);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              const int e = 8 * j + 2 * h;
+              w[h] = f2_to_e4m3x2(__fmul_rn(lo_f(acc[e]), inv), __fmul_rn(hi_f(acc[e]), inv)) |
+                     (f2_to_e4m3x2(__fmul_rn(lo_f(acc[e + 1]), inv), __fmul_rn(hi_f(acc[e + 1]), inv)) << 16);
+            }
+            dst[j] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        named_bar_sync(1, 256);  // amax_x is free for the next tile
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, Cfg::kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------- few rows per expert
+// Swap-AB as in bs_decode.cuh: the weight block's 128 rows are the MMA's M, up to NT output rows ("tokens") its N. A
+// cluster of S CTAs takes a tile together: CTA j of it streams the j-th 1/S of the K blocks, then every CTA sends its
+// fp32 partial of token tt to CTA tt % S through distributed shared memory, which adds the S partials in CTA order and
+// finishes its tokens. So a call with few tiles still uses every SM, the sum's order is fixed, and no partial goes
+// through global memory.
+//
+// CTA layout (384 threads): warps 0-7 promotion (warpgroup g: tokens [g * NT/2, ...)) and epilogue, warp 8 TMA
+// producer, warp 9 TMEM + MMA issuer, warps 10-11 scale products As[src, kb] * Bs[nb, kb] into a ring of eight slots.
+template <bool FUSED, int NT>
+struct GroupedTokensCfg {
+  static constexpr int kThreads = 384;
+  static constexpr int kNwg = FUSED ? 2 : 1;
+  static constexpr int kTr = NT / 2;
+  static constexpr int kWBytes = 16384 * kNwg;
+  static constexpr int kXBytes = NT * 128;
+  static constexpr int kStageBytes = kWBytes + ((kXBytes + 1023) / 1024) * 1024;
+  static constexpr int kBufCols = kNwg * NT;
+  static constexpr int kBufs = 512 / kBufCols > 4 ? 4 : 512 / kBufCols;
+  static constexpr int kTmemCols = kBufs * kBufCols < 32 ? 32 : kBufs * kBufCols;
+  static_assert((kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols <= 512, "TMEM columns");
+  static constexpr int kSlots = 8;
+  static constexpr int kRingBytes = kSlots * kNwg * NT * 4;
+  static constexpr int kXchBytes = kNwg * NT * 128 * 4;     // [S][kNwg][NT / S][128] partials
+  static constexpr int kAmaxBytes = FUSED ? NT * 4 * 4 : 0;  // [own token][4 warps]
+  static constexpr int kBarBytes = 512;
+  static constexpr int kTail = kRingBytes + kXchBytes + kAmaxBytes + kBarBytes + static_cast<int>(sizeof(GroupTable));
+  static constexpr int kStagesRaw = (232448 - 1024 - kTail) / kStageBytes;
+  static constexpr int kStages = kStagesRaw > 10 ? 10 : kStagesRaw;
+  static_assert(kStages >= 3, "pipeline depth");
+  static constexpr int kXchOff = kStages * kStageBytes;
+  static constexpr int kRingOff = kXchOff + kXchBytes;
+  static constexpr int kAmaxOff = kRingOff + kRingBytes;
+  static constexpr int kBarOff = kAmaxOff + kAmaxBytes;
+  static constexpr int kTableOff = kBarOff + kBarBytes;
+  static constexpr int kUsed = kTableOff + static_cast<int>(sizeof(GroupTable));
+  // more than half of the SM's shared memory, so that a second CTA (and its TMEM) never lands on the SM
+  static constexpr int kSmemBytes = (kUsed > 120 * 1024 ? kUsed : 120 * 1024) + 1024;
+};
+
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+// Arrival on a barrier of any CTA of the cluster; publishes this thread's earlier writes (and what it has seen) there.
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// mbar_wait_warp that also acquires what CTAs of the cluster published.
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort, int* status) {
+  if (__all_sync(0xffffffffu, mbar_try_wait_cluster(bar, parity))) return true;
+  const uint64_t t0 = globaltimer_ns();
+  uint32_t spins = 0;
+  while (true) {
+    if (__all_sync(0xffffffffu, mbar_try_wait_cluster(bar, parity))) return true;
+    if ((spins++ & 63u) == 0) {
+      const bool late = globaltimer_ns() - t0 > kWaitLimitNs;
+      if (late) {
+        atomicCAS(status, 0, kErrTimeoutCluster);
+        *abort = 1;
+      }
+      if (__any_sync(0xffffffffu, late || *abort)) return false;
+    }
+  }
+}
+
+// log_s: log2 of the cluster size S (1, 2, 4, 8).
+template <bool FUSED, int NT>
+__global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
+    k_grouped_tokens(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                     const GroupedParams p, const int log_s) {
+  using Cfg = GroupedTokensCfg<FUSED, NT>;
+  constexpr int ST = Cfg::kStages, NWG = Cfg::kNwg, NB = Cfg::kBufs, NS = Cfg::kSlots, TR = Cfg::kTr;
+  extern __shared__ uint8_t smem_raw[];
+  // (the offset of the aligned base is the same in every CTA: mapped addresses of the cluster's CTAs agree)
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* xch = reinterpret_cast<float*>(smem + Cfg::kXchOff);
+  float* ring = reinterpret_cast<float*>(smem + Cfg::kRingOff);  // [NS][NWG][NT] scale products
+  float* amx = reinterpret_cast<float*>(smem + Cfg::kAmaxOff);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::kBarOff);
+  uint64_t* empty = full + ST;
+  uint64_t* pfull = empty + ST;
+  uint64_t* pempty = pfull + NB;
+  uint64_t* sfull = pempty + NB;
+  uint64_t* sempty = sfull + NS;
+  uint64_t* drain = sempty + NS;
+  uint64_t* rfull = drain + 1;   // every CTA's partials of this CTA's tokens are here
+  uint64_t* rempty = rfull + 1;  // every CTA has read the partials of the previous tile
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rempty + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert((2 * ST + 2 * NB + 2 * NS + 3) * 8 + 8 <= Cfg::kBarBytes, "barrier area");
+  GroupTable& table = *reinterpret_cast<GroupTable*>(smem + Cfg::kTableOff);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int S = 1 << log_s;
+  const int rank = static_cast<int>(cluster_ctarank());
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < NB; ++i) {
+      mbar_init(&pfull[i], 1);
+      mbar_init(&pempty[i], 256);
+    }
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&sfull[i], 64);
+      mbar_init(&sempty[i], 256);
+    }
+    mbar_init(drain, 1);
+    mbar_init(rfull, 8 * S);
+    mbar_init(rempty, 8 * S);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmX);
+    grid_dep_launch();
+  }
+  const int KB = p.KB, nblk = p.nblk;
+  const int I_blk = FUSED ? nblk / 2 : 0;
+  const int num_n = FUSED ? I_blk : nblk;
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, Cfg::kTmemCols);
+    tmem_relinquish();
+  }
+  grid_dep_wait();
+  if (warp == 0) build_table(table, p, NT, num_n);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // every CTA's barriers exist before a remote arrival
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int num_tiles = table.tiles;
+  const int first = static_cast<int>(blockIdx.x) >> log_s, step = static_cast<int>(gridDim.x) >> log_s;
+  const int kb0 = KB * rank >> log_s, kb1 = KB * (rank + 1) >> log_s;
+
+  if (warp == 8) {
+    // ------------------------------------------------------------ TMA producer
+    const uint64_t pol_w = policy_evict_first(), pol_x = policy_evict_last();
+    const bool gather = p.row_token != nullptr;
+    int s = 0;
+    uint32_t ph = 0, issued = 0, parity_bits = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < num_tiles; tile += step) {
+      const GroupTile t = find_tile(table, tile, NT);
+      const int quads = (t.rows + 3) / 4;
+      int4 rows = make_int4(0, 0, 0, 0);
+      if (gather && lane < quads) {
+        const int last = t.row + t.rows - 1, r = t.row + 4 * lane;
+        rows = make_int4(source_row(p, r), source_row(p, min(r + 1, last)), source_row(p, min(r + 2, last)),
+                         source_row(p, min(r + 3, last)));
+      }
+      const int nb = t.expert * nblk + t.tn;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (lane == 0) ok = mbar_wait(&empty[s], ph ^ 1, abort_flag, p.status, kErrTimeoutEmpty);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        uint8_t* st = smem + s * Cfg::kStageBytes;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&full[s], Cfg::kWBytes + (gather ? quads * 512 : Cfg::kXBytes));
+#pragma unroll
+          for (int w = 0; w < NWG; ++w)
+            load_weight_box(st + w * 16384, &tmW, &full[s], w == 0 ? nb : nb + I_blk, kb, KB, p.b_tiled, pol_w);
+          if (!gather) tma_load_2d(st + Cfg::kWBytes, &tmX, &full[s], kb * 128, t.row, pol_x);
+        }
+        __syncwarp();
+        if (gather && lane < quads) tma_gather4(st + Cfg::kWBytes + 512 * lane, &tmX, &full[s], kb * 128, rows, pol_x);
+        issued |= 1u << s;
+        parity_bits = (parity_bits & ~(1u << s)) | (ph << s);
+        if (++s == ST) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    if (!ok && lane == 0)
+      for (int i = 0; i < ST; ++i)
+        if (issued & (1u << i))
+          mbar_wait(&full[i], (parity_bits >> i) & 1u, abort_flag, p.status, kErrTimeoutDrain, 100000000ull);
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      int s = 0, b = 0;
+      uint32_t ph = 0, pph = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < num_tiles; tile += step) {
+        const GroupTile t = find_tile(table, tile, NT);
+        // Columns past the tile's rows are computed from whatever the stage holds (or skipped) and never read.
+        const uint32_t idesc = idesc_e4m3_f32(128, (t.rows + 15) / 16 * 16);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = mbar_wait(&full[s], ph, abort_flag, p.status, kErrTimeoutFull) &&
+               mbar_wait(&pempty[b], pph ^ 1, abort_flag, p.status, kErrTimeoutPEmpty);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t st = smem_u32(smem + s * Cfg::kStageBytes);
+          const uint32_t xs = st + Cfg::kWBytes;
+#pragma unroll
+          for (int w = 0; w < NWG; ++w) {
+            const uint32_t d = tmem + static_cast<uint32_t>(b * Cfg::kBufCols + w * NT);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mma_e4m3(d, desc_kmajor_sw128(st + w * 16384 + 32 * k), desc_kmajor_sw128(xs + 32 * k), idesc,
+                       k > 0 ? 1u : 0u);
+          }
+          mma_commit(&empty[s]);
+          mma_commit(&pfull[b]);
+          if (++s == ST) {
+            s = 0;
+            ph ^= 1;
+          }
+          if (++b == NB) {
+            b = 0;
+            pph ^= 1;
+          }
+        }
+      }
+      mma_commit(drain);
+      mbar_wait(drain, 0, abort_flag, p.status, kErrTimeoutDrain, 100000000ull);
+    }
+  } else if (warp >= 10) {
+    // ------------------------------------------------------------ scale products
+    constexpr int TPL = (NT + 63) / 64;
+    const int tok_base = (warp - 10) * 32 * TPL + lane;
+    int slot = 0;
+    uint32_t sph = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < num_tiles; tile += step) {
+      const GroupTile t = find_tile(table, tile, NT);
+      const float* arow[TPL];
+#pragma unroll
+      for (int j = 0; j < TPL; ++j) {
+        const int tok = tok_base + 32 * j;
+        arow[j] = p.As + static_cast<size_t>(source_row(p, t.row + (tok < t.rows ? tok : 0))) * KB;
+      }
+      const float* brow = p.Bs + (static_cast<size_t>(t.expert) * nblk + t.tn) * KB;
+      const float* urow = brow + static_cast<size_t>(I_blk) * KB;
+      float a[2][TPL], bw[2][NWG];  // operands of this K block and the next
+      auto load = [&](int h, int kb) {
+#pragma unroll
+        for (int j = 0; j < TPL; ++j) a[h][j] = ldg_f32(arow[j] + kb);
+#pragma unroll
+        for (int w = 0; w < NWG; ++w) bw[h][w] = ldg_f32((w == 0 ? brow : urow) + kb);
+      };
+      auto write = [&](int h, int kb_next) {
+        if (!mbar_wait(&sempty[slot], sph ^ 1, abort_flag, p.status, kErrTimeoutPEmpty)) {
+          ok = false;
+          return;
+        }
+        float* dst = ring + slot * (NWG * NT);
+#pragma unroll
+        for (int w = 0; w < NWG; ++w)
+#pragma unroll
+          for (int j = 0; j < TPL; ++j) {
+            const int tok = tok_base + 32 * j;
+            if (tok < NT) dst[w * NT + tok] = tok < t.rows ? __fmul_rn(a[h][j], bw[h][w]) : 0.f;
+          }
+        mbar_arrive(&sfull[slot]);
+        load(h, kb_next);
+        if (++slot == NS) {
+          slot = 0;
+          sph ^= 1;
+        }
+      };
+      if (kb0 < kb1) {
+        load(0, kb0);
+        load(1, min(kb0 + 1, kb1 - 1));
+      }
+      for (int kb = kb0; kb < kb1 && ok; kb += 2) {
+        write(0, min(kb + 2, kb1 - 1));
+        if (kb + 1 < kb1 && ok) write(1, min(kb + 3, kb1 - 1));
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ promotion + epilogue
+    const int wg = warp >> 2;
+    const int q = warp & 3;
+    const int tok0 = wg * TR;
+    const int r = q * 32 + lane;  // weight row inside the block
+    const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
+    const int own = NT >> log_s;  // tokens a CTA finishes
+    int b = 0, slot = 0;
+    uint32_t pph = 0, sph = 0, rph = 0;
+    bool ok = true;
+    for (int tile = first; tile < num_tiles; tile += step) {
+      const GroupTile t = find_tile(table, tile, NT);
+      const int n = t.rows;
+      uint64_t acc[NWG][TR / 2];
+#pragma unroll
+      for (int w = 0; w < NWG; ++w)
+#pragma unroll
+        for (int i = 0; i < TR / 2; ++i) acc[w][i] = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (ok && !(mbar_wait_warp(&pfull[b], pph, abort_flag, p.status, kErrTimeoutPFull) &&
+                    mbar_wait_warp(&sfull[slot], sph, abort_flag, p.status, kErrTimeoutPFull)))
+          ok = false;
+        if (ok) {
+          tc_fence_after();
+          const uint32_t tb = tmem + lane_addr + static_cast<uint32_t>(b * Cfg::kBufCols + tok0);
+          const ulonglong2* sc = reinterpret_cast<const ulonglong2*>(ring + slot * (NWG * NT) + tok0);
+          constexpr int CH = TR < 16 ? TR : 16;  // columns skipped together when the tile has no such tokens
+          uint32_t v[NWG][TR];
+#pragma unroll
+          for (int c0 = 0; c0 < TR; c0 += CH)
+            if (tok0 + c0 < n) {
+#pragma unroll
+              for (int w = 0; w < NWG; ++w) tmem_ld_run<CH>(tb + w * NT + c0, v[w] + c0);
+            }
+          tmem_ld_wait();
+          mbar_arrive(&pempty[b]);
+#pragma unroll
+          for (int c0 = 0; c0 < TR; c0 += CH)
+            if (tok0 + c0 < n) {
+#pragma unroll
+              for (int w = 0; w < NWG; ++w)
+#pragma unroll
+                for (int i = c0; i < c0 + CH; i += 4) {
+                  const ulonglong2 s2 = sc[(w * NT + i) / 4];
+                  ffma2(acc[w][i / 2], v[w][i], v[w][i + 1], s2.x);
+                  ffma2(acc[w][i / 2 + 1], v[w][i + 2], v[w][i + 3], s2.y);
+                }
+            }
+          mbar_arrive(&sempty[slot]);
+        }
+        if (++b == NB) {
+          b = 0;
+          pph ^= 1;
+        }
+        if (++slot == NS) {
+          slot = 0;
+          sph ^= 1;
+        }
+      }
+
+      // ---------------- partials to the tokens' owners
+      if (ok && !mbar_wait_cluster(rempty, rph ^ 1, abort_flag, p.status)) ok = false;
+      if (ok) {
+#pragma unroll
+        for (int i = 0; i < TR; ++i) {
+          const int tok = tok0 + i;
+          if (tok < n) {
+            const int to = tok & (S - 1);
+#pragma unroll
+            for (int w = 0; w < NWG; ++w)
+              st_cluster_f32(mapa_shared(xch + ((rank * NWG + w) * own + (tok >> log_s)) * 128 + r, to),
+                             (i & 1) ? hi_f(acc[w][i / 2]) : lo_f(acc[w][i / 2]));
+          }
+        }
+        __syncwarp();
+        if (lane < S) mbar_arrive_cluster(mapa_shared(rfull, lane));
+        if (!mbar_wait_cluster(rfull, rph, abort_flag, p.status)) ok = false;
+      }
+      // ---------------- this CTA's tokens: rank, rank + S, ... below n
+      const int n_own = n > rank ? (n - rank + S - 1) >> log_s : 0;
+      if constexpr (!FUSED) {
+        if (ok) {
+          for (int j = warp; j < n_own; j += 8) {
+            float4 c = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int s = 0; s < S; ++s) {
+              const float4 v = *reinterpret_cast<const float4*>(xch + (s * own + j) * 128 + lane * 4);
+              c.x += v.x, c.y += v.y, c.z += v.z, c.w += v.w;
+            }
+            const size_t at = static_cast<size_t>(t.row + (j << log_s) + rank) * p.ldc + static_cast<size_t>(t.tn) * 128 + lane * 4;
+            if (p.out_f32)
+              *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = c;
+            else
+              *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + at) =
+                  make_uint2(pack_bf16x2(c.x, c.y), pack_bf16x2(c.z, c.w));
+          }
+        }
+      } else {
+        // y = silu(g) * u per (token, weight row), kept in this thread's own word of the gate partial; the group's
+        // amax is a warp maximum (|y| orders like its bits) and four warps' through shared memory.
+        if (ok) {
+          for (int j = wg; j < n_own; j += 2) {
+            float g = 0.f, u = 0.f;
+            for (int s = 0; s < S; ++s) {
+              g += xch[((s * 2 + 0) * own + j) * 128 + r];
+              u += xch[((s * 2 + 1) * own + j) * 128 + r];
+            }
+            const float y = silu_mul(g, u);
+            xch[j * 128 + r] = y;
+            const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(y)));
+            if (lane == 0) amx[j * 4 + q] = __uint_as_float(m);
+          }
+        }
+        named_bar_sync(1 + wg, 128);
+        if (ok) {
+          for (int j = wg + 2 * q; j < n_own; j += 8) {
+            const float4 a4 = *reinterpret_cast<const float4*>(amx + j * 4);
+            const float amax = fmaxf(fmaxf(a4.x, a4.y), fmaxf(a4.z, a4.w));
+            const float scale = __fdiv_rn(fmaxf(amax, 1e-10f), 448.0f);
+            const float inv = __fdiv_rn(1.0f, scale);
+            const size_t row = static_cast<size_t>(t.row + (j << log_s) + rank);
+            if (lane == 0) p.qs[row * I_blk + t.tn] = scale;
+            const float4 y = *reinterpret_cast<const float4*>(xch + j * 128 + lane * 4);
+            *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.out) + (row * I_blk + t.tn) * 128 + lane * 4) =
+                f2_to_e4m3x2(__fmul_rn(y.x, inv), __fmul_rn(y.y, inv)) |
+                (f2_to_e4m3x2(__fmul_rn(y.z, inv), __fmul_rn(y.w, inv)) << 16);
+          }
+        }
+      }
+      if (ok) {
+        __syncwarp();
+        if (lane < S) mbar_arrive_cluster(mapa_shared(rempty, lane));
+      }
+      rph ^= 1;
+    }
+  }
+  // No CTA leaves while another of its cluster may still write to it or arrive on its barriers.
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 9) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, Cfg::kTmemCols);
+  }
+}
+
+}  // namespace bs

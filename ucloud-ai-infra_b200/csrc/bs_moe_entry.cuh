@@ -1,0 +1,272 @@
+// C-ABI entry points of the mixture-of-experts operators: argument checks, kernel selection and launch. Part of
+// bs_capi.cu's translation unit (its helpers and the status word).
+#pragma once
+
+namespace {
+
+// Tokens per CTA of the route kernels: one round of a CTA's warps, more when that would take more CTAs than SMs
+// (k_moe_place reads every CTA's counts).
+int route_tokens_per_cta(int T, int num_sms) {
+  const int rounds = (T + bs::kRouteFuse * num_sms - 1) / (bs::kRouteFuse * num_sms);
+  return bs::kRouteFuse * (rounds > 1 ? rounds : 1);
+}
+int route_grid(int T, int num_sms) {
+  const int per = route_tokens_per_cta(T, num_sms);
+  return T > 0 ? (T + per - 1) / per : 1;
+}
+
+template <int VPL>
+int launch_route(const bs::RouteParams& p, int f32, int grid, cudaStream_t s) {
+  int rc = launch_pdl(bs::k_moe_route<VPL>, grid, bs::kRouteThreads, 0, s, "k_moe_route launch", p, f32);
+  if (rc == BS_OK && grid > 1) rc = launch_pdl(bs::k_moe_place, grid, bs::kRouteThreads, 0, s, "k_moe_place launch", p);
+  return rc;
+}
+
+int run_route(bs::RouteParams& p, int f32, void* scratch, size_t scratch_bytes, void* stream) {
+  if (p.T < 0 || p.k <= 0 || p.k > bs::kMaxTopK || p.E <= 0 || p.E > bs::kMaxExperts) return BS_ERR_ARG;
+  if (p.e_begin < 0 || p.e_count <= 0 || p.e_count > p.E - p.e_begin) return BS_ERR_ARG;
+  if (static_cast<long long>(p.T) * p.k >= (1ll << 31)) return BS_ERR_ARG;
+  if (!p.offsets || (p.T > 0 && (!p.row_token || !p.slot_row))) return BS_ERR_ARG;
+  DeviceState* d = device_state();
+  if (!d) return BS_ERR_CUDA;
+  p.per_cta = route_tokens_per_cta(p.T, d->num_sms);
+  const int grid = route_grid(p.T, d->num_sms);
+  if (grid > 1) {
+    if (!scratch || scratch_bytes < static_cast<size_t>(grid) * p.e_count * sizeof(int)) return BS_ERR_WORKSPACE;
+    if (reinterpret_cast<uintptr_t>(scratch) & 3u) return BS_ERR_ALIGN;
+    p.hist = static_cast<int*>(scratch);
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (!p.logits) return launch_route<0>(p, 0, grid, s);
+  if (p.E <= 32) return launch_route<1>(p, f32, grid, s);
+  if (p.E <= 64) return launch_route<2>(p, f32, grid, s);
+  if (p.E <= 128) return launch_route<4>(p, f32, grid, s);
+  if (p.E <= 256) return launch_route<8>(p, f32, grid, s);
+  return launch_route<16>(p, f32, grid, s);
+}
+
+// How a grouped product runs.
+struct GroupedPlan {
+  int nt;     // rows per tile of k_grouped_tokens; 0: k_grouped_rows
+  int log_s;  // k_grouped_tokens: log2 of the CTAs per tile
+};
+
+GroupedPlan grouped_plan(bool fused, int E, int nblk, int KB, int rows, int num_sms) {
+  GroupedPlan g = {0, 0};
+  const int mean = (rows + E - 1) / E;
+  g.nt = mean <= 12 ? 16 : mean <= 28 ? 32 : mean <= 64 ? 64 : 0;
+  if (!g.nt) return g;
+  const int active = rows < E ? rows : E;
+  const int tiles = active * (fused ? nblk / 2 : nblk);
+  while (g.log_s < 3 && (2 << g.log_s) <= KB && (tiles << g.log_s) < 4 * num_sms) ++g.log_s;
+  return g;
+}
+
+template <bool FUSED, int NT>
+int launch_grouped_tokens(const CUtensorMap& tmW, const CUtensorMap& tmX, const bs::GroupedParams& p, int log_s,
+                          int num_sms, cudaStream_t s) {
+  using Cfg = bs::GroupedTokensCfg<FUSED, NT>;
+  constexpr auto kern = bs::k_grouped_tokens<FUSED, NT>;
+  const int rc = prepare_kernel<kern>(Cfg::kSmemBytes, 0);
+  if (rc != BS_OK) return rc;
+  const int clusters = max_clusters<kern>(Cfg::kThreads, Cfg::kSmemBytes, log_s, num_sms);
+  if (clusters <= 0) return BS_ERR_CUDA;
+  return launch_pdl_cluster(kern, clusters << log_s, Cfg::kThreads, Cfg::kSmemBytes, 1 << log_s, s,
+                            "k_grouped_tokens launch", tmW, tmX, p, log_s);
+}
+
+template <bool FUSED>
+int run_grouped(const void* A, const void* B, const bs::GroupedParams& p, int rows_hint, cudaStream_t s, int num_sms) {
+  const int K = p.KB * 128;
+  const GroupedPlan g = grouped_plan(FUSED, p.E, p.nblk, p.KB, rows_hint, num_sms);
+  const bool gather = p.row_token != nullptr;
+  CUtensorMap tmA, tmB;
+  if (make_weight_map(&tmB, B, p.E * p.nblk * 128, K, p.b_tiled, FUSED && !g.nt ? 64 : 128) != BS_OK) return BS_ERR_TMAP;
+  if (make_map(&tmA, A, K, p.rows_a, K, 128, gather ? 1 : g.nt ? g.nt : 128) != BS_OK) return BS_ERR_TMAP;
+  switch (g.nt) {
+    case 16: return launch_grouped_tokens<FUSED, 16>(tmB, tmA, p, g.log_s, num_sms, s);
+    case 32: return launch_grouped_tokens<FUSED, 32>(tmB, tmA, p, g.log_s, num_sms, s);
+    case 64: return launch_grouped_tokens<FUSED, 64>(tmB, tmA, p, g.log_s, num_sms, s);
+    default: break;
+  }
+  using Cfg = bs::GroupedRowsCfg<FUSED>;
+  constexpr auto kern = bs::k_grouped_rows<FUSED>;
+  const int rc = prepare_kernel<kern>(Cfg::kSmemBytes, Cfg::Regs::kLaunch);
+  if (rc != BS_OK) return rc;
+  return launch_pdl(kern, num_sms, Cfg::kThreads, Cfg::kSmemBytes, s, "k_grouped_rows launch", tmA, tmB, p);
+}
+
+int validate_grouped(const void* A, const void* B, const void* out, const float* As, const float* Bs, const float* qs,
+                     const int* offsets, const int* row_token, int rows_a, int R, int rows_hint, int E, int N, int K,
+                     int ldc, int b_tiled, int out_dtype, bool fused) {
+  if (rows_a < 0 || R < 0 || rows_hint < 0 || rows_hint > R || E <= 0 || E > bs::kMaxExperts) return BS_ERR_ARG;
+  const int rc = validate_gemm(fused, A, B, out, As, Bs, qs, R, N, K, ldc, b_tiled, out_dtype);
+  if (rc != BS_OK || R == 0) return rc;
+  if (!offsets || rows_a == 0 || (!row_token && rows_a < R)) return BS_ERR_ARG;
+  // 32-bit tile counts and TMA coordinates
+  if (static_cast<long long>(E) * N * (b_tiled ? K / 128 : 1) >= (1ll << 31)) return BS_ERR_ARG;
+  if ((static_cast<long long>(R) / 16 + E) * (N / 128) >= (1ll << 31)) return BS_ERR_ARG;
+  return BS_OK;
+}
+
+bs::GroupedParams grouped_params(const float* As, const float* Bs, const int* offsets, const int* row_token, int rows_a,
+                                 int R, int E, int N, int K, int b_tiled, int* status) {
+  bs::GroupedParams p = {};
+  p.E = E;
+  p.R = R;
+  p.rows_a = rows_a;
+  p.nblk = N / 128;
+  p.KB = K / 128;
+  p.b_tiled = b_tiled;
+  p.offsets = offsets;
+  p.row_token = row_token;
+  p.As = As;
+  p.Bs = Bs;
+  p.status = status;
+  return p;
+}
+
+template <int C>
+int launch_block(const bs::BlockParams& p, bool wide, int threads, int num_sms, cudaStream_t s) {
+  auto kern = wide ? bs::k_block_norm<C, true> : bs::k_block_norm<C, false>;
+  int per_sm = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, 0) != cudaSuccess || per_sm < 1) per_sm = 1;
+  cudaGetLastError();
+  const int grid = p.T < per_sm * num_sms ? p.T : per_sm * num_sms;
+  return launch_pdl(kern, grid, threads, 0, s, "k_block_norm launch", p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int bs_fp8_moe_route(const void* logits, int dtype, long long ldl, int T, int n_experts, int top_k, int renormalize,
+                     float scale, int e_begin, int e_count, float* weights, int* ids, int* offsets, int* row_token,
+                     int* slot_row, void* scratch, size_t scratch_bytes, void* stream) {
+  if ((dtype != 0 && dtype != 1) || ldl < n_experts || top_k > n_experts) return BS_ERR_ARG;
+  if (T > 0 && (!logits || !weights || !ids)) return BS_ERR_ARG;
+  if (reinterpret_cast<uintptr_t>(logits) & (dtype ? 3u : 1u)) return BS_ERR_ALIGN;
+  bs::RouteParams p = {};
+  static const float none = 0.f;  // T == 0: a pointer that says "logits", never read
+  p.logits = logits ? logits : &none;
+  p.ldl = ldl;
+  p.T = T;
+  p.E = n_experts;
+  p.k = top_k;
+  p.renormalize = renormalize;
+  p.scale = scale;
+  p.e_begin = e_begin;
+  p.e_count = e_count;
+  p.weights = weights;
+  p.ids = ids;
+  p.offsets = offsets;
+  p.row_token = row_token;
+  p.slot_row = slot_row;
+  return run_route(p, dtype, scratch, scratch_bytes, stream);
+}
+
+int bs_fp8_moe_dispatch(const int* ids, int T, int n_experts, int top_k, int e_begin, int e_count, int* offsets,
+                        int* row_token, int* slot_row, void* scratch, size_t scratch_bytes, void* stream) {
+  if (T > 0 && !ids) return BS_ERR_ARG;
+  bs::RouteParams p = {};
+  p.ids_in = ids;
+  p.T = T;
+  p.E = n_experts;
+  p.k = top_k;
+  p.e_begin = e_begin;
+  p.e_count = e_count;
+  p.offsets = offsets;
+  p.row_token = row_token;
+  p.slot_row = slot_row;
+  return run_route(p, 0, scratch, scratch_bytes, stream);
+}
+
+size_t bs_fp8_moe_scratch_bytes(int T, int e_count) {
+  if (T <= 0 || e_count <= 0) return 0;
+  DeviceState* d = device_state();
+  const int grid = route_grid(T, d ? d->num_sms : 148);
+  return grid > 1 ? static_cast<size_t>(grid) * e_count * sizeof(int) : 0;
+}
+
+int bs_fp8_grouped_gemm(const void* A, const void* B, void* C, const float* As, const float* Bs, const int* offsets,
+                        const int* row_token, int rows_a, int R, int rows_hint, int E, int N, int K, int ldc,
+                        int b_tiled, int out_dtype, void* stream) {
+  const int rc = validate_grouped(A, B, C, As, Bs, nullptr, offsets, row_token, rows_a, R, rows_hint, E, N, K, ldc,
+                                  b_tiled, out_dtype, false);
+  if (rc != BS_OK || R == 0) return rc;
+  DeviceState* d = device_state();
+  if (!d) return BS_ERR_CUDA;
+  bs::GroupedParams p = grouped_params(As, Bs, offsets, row_token, rows_a, R, E, N, K, b_tiled, d->status);
+  p.ldc = ldc;
+  p.out_f32 = out_dtype;
+  p.out = C;
+  return run_grouped<false>(A, B, p, rows_hint ? rows_hint : R, static_cast<cudaStream_t>(stream), d->num_sms);
+}
+
+int bs_fp8_grouped_gemm_silu_quant(const void* A, const void* B, void* Q, const float* As, const float* Bs, float* Qs,
+                                   const int* offsets, const int* row_token, int rows_a, int R, int rows_hint, int E,
+                                   int N2, int K, int b_tiled, void* stream) {
+  const int rc = validate_grouped(A, B, Q, As, Bs, Qs, offsets, row_token, rows_a, R, rows_hint, E, N2, K, N2 / 2,
+                                  b_tiled, 0, true);
+  if (rc != BS_OK || R == 0) return rc;
+  DeviceState* d = device_state();
+  if (!d) return BS_ERR_CUDA;
+  bs::GroupedParams p = grouped_params(As, Bs, offsets, row_token, rows_a, R, E, N2, K, b_tiled, d->status);
+  p.ldc = N2 / 2;
+  p.out = Q;
+  p.qs = Qs;
+  return run_grouped<true>(A, B, p, rows_hint ? rows_hint : R, static_cast<cudaStream_t>(stream), d->num_sms);
+}
+
+int bs_fp8_block_norm_quant(const void* y, long long ldy, int rows_y, const float* weights, const int* slot_row,
+                            int top_k, const void* residual, long long ldr, void* out, long long ldo, int wide,
+                            const void* post_weight, const void* gate, int gate_kind, long long ldg, float scale,
+                            float residual_scale, const void* pre_weight, float eps, void* A, float* As, int T, int H,
+                            void* stream) {
+  if (T < 0 || H <= 0 || H % 128 || H > bs::kBlockMaxThreads * bs::kBlockMaxChunks * 8) return BS_ERR_ARG;
+  if (wide != 0 && wide != 1) return BS_ERR_ARG;
+  const int per16 = wide ? 4 : 8;  // elements of the residual per 16 bytes
+  if (ldy < H || ldy % 8 || ldr < H || ldr % per16 || ldo < H || ldo % per16 || rows_y < 0) return BS_ERR_ARG;
+  if (!(eps >= 0.f) || gate_kind < 0 || gate_kind > 3 || (gate_kind != 0) != (gate != nullptr)) return BS_ERR_ARG;
+  if ((gate_kind == 3 && (ldg < H || ldg % 8)) || (gate_kind == 2 && ldg < 1)) return BS_ERR_ARG;
+  if ((weights == nullptr) != (slot_row == nullptr) || (weights && top_k <= 0) || (!weights && rows_y < T)) return BS_ERR_ARG;
+  if (T == 0) return BS_OK;
+  if (!y || !residual || !out || (pre_weight && (!A || !As))) return BS_ERR_ARG;
+  if (!aligned16(y) || !aligned16(residual) || !aligned16(out) || !aligned16(post_weight) || !aligned16(pre_weight) ||
+      !aligned16(A) || (gate_kind != 2 && !aligned16(gate)))
+    return BS_ERR_ALIGN;
+  DeviceState* d = device_state();
+  if (!d) return BS_ERR_CUDA;
+  bs::BlockParams p = {};
+  p.y = static_cast<const __nv_bfloat16*>(y);
+  p.ldy = ldy;
+  p.rows_y = rows_y;
+  p.weights = weights;
+  p.slot_row = slot_row;
+  p.k = top_k;
+  p.residual = residual;
+  p.ldr = ldr;
+  p.out = out;
+  p.ldo = ldo;
+  p.post = static_cast<const __nv_bfloat16*>(post_weight);
+  p.gate = static_cast<const __nv_bfloat16*>(gate);
+  p.gate_kind = gate_kind;
+  p.ldg = ldg;
+  p.scale = scale;
+  p.residual_scale = residual_scale;
+  p.pre = static_cast<const __nv_bfloat16*>(pre_weight);
+  p.eps = eps;
+  p.A = static_cast<uint8_t*>(A);
+  p.As = As;
+  p.T = T;
+  p.H = H;
+  const int chunks = H / 8;
+  const int c = chunks <= bs::kBlockMaxThreads ? 1 : chunks <= 2 * bs::kBlockMaxThreads ? 2 : 4;
+  const int threads = ((chunks + c - 1) / c + 31) / 32 * 32;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (c == 1) return launch_block<1>(p, wide != 0, threads, d->num_sms, s);
+  if (c == 2) return launch_block<2>(p, wide != 0, threads, d->num_sms, s);
+  return launch_block<4>(p, wide != 0, threads, d->num_sms, s);
+}
+
+}  // extern "C"

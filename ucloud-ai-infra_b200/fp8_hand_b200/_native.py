@@ -25,6 +25,7 @@ BS_ERR_TIMEOUT_SELFTEST = 199
 
 # (name, restype, argtypes) for every symbol of include/bs_fp8.h
 _VP, _I, _SZ, _U64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_uint64
+_LL, _F = ctypes.c_longlong, ctypes.c_float
 SIGNATURES = {
     "bs_fp8_gemm": (_I, [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _VP, _SZ, _VP]),
     "bs_fp8_gemm_silu_quant": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _VP, _SZ, _VP]),
@@ -37,6 +38,13 @@ SIGNATURES = {
     "bs_fp8_silu_mul": (_I, [_VP, _I, _VP, _I, _I, _I, _VP]),
     "bs_fp8_tp_reduce_switch": (_I, [_U64, _VP, _U64, ctypes.c_longlong, _I, _I, ctypes.c_uint, _U64, _VP]),
     "bs_fp8_tp_flag_words": (ctypes.c_longlong, [_I]),
+    "bs_fp8_moe_route": (_I, [_VP, _I, _LL, _I, _I, _I, _I, _F, _I, _I, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "bs_fp8_moe_dispatch": (_I, [_VP, _I, _I, _I, _I, _I, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "bs_fp8_moe_scratch_bytes": (_SZ, [_I, _I]),
+    "bs_fp8_grouped_gemm": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _I, _I, _VP]),
+    "bs_fp8_grouped_gemm_silu_quant": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _VP]),
+    "bs_fp8_block_norm_quant": (_I, [_VP, _LL, _I, _VP, _VP, _I, _VP, _LL, _VP, _LL, _I, _VP, _VP, _I, _LL, _F, _F,
+                                     _VP, _F, _VP, _VP, _I, _I, _VP]),
     "bs_fp8_status": (_I, [ctypes.POINTER(_I), _I]),
     "bs_fp8_selftest_wait_timeout": (_I, [_U64, _VP]),
     "bs_fp8_launch_plan": (_I, [_I, _I, _I, _I, ctypes.POINTER(_I), _I]),

@@ -7,12 +7,16 @@ failure raises RuntimeError.
 """
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
 
 from . import _native
 
 E4M3 = torch.float8_e4m3fn
 BLOCK = 128
+MAX_EXPERTS = 512
+MAX_TOP_K = 32
 
 
 def _need(cond: bool, msg: str) -> None:
@@ -228,3 +232,232 @@ def gemm_silu_quant(A: torch.Tensor, B: torch.Tensor, As: torch.Tensor, Bs: torc
             M, N2, K, int(b_tiled), _native.ptr(ws), 0 if ws is None else ws.numel(),
             _native.stream_handle(dev)), "bs_fp8_gemm_silu_quant")
     return Q, Qs
+
+
+# ------------------------------------------------------------------ mixture of experts
+@dataclass(slots=True)
+class MoeRoute:
+    """A routed batch of T tokens with k slots each (moe_route, moe_dispatch), all on the device. Rows are the
+    (token, slot) pairs whose expert is local, sorted by expert and then by place in ids.
+
+      weights    fp32 [T, k]           weight of each slot
+      ids        int32 [T, k]          expert of each slot, -1 for none
+      offsets    int32 [experts + 1]   rows of local expert e: offsets[e] .. offsets[e + 1] - 1
+      row_token  int32 [T * k]         token of each row, -1 past offsets[-1]
+      slot_row   int32 [T, k]          row of each slot, -1 when its expert is not local
+      num_experts  experts in all (None: the local ones)
+    """
+    weights: torch.Tensor | None
+    ids: torch.Tensor
+    offsets: torch.Tensor
+    row_token: torch.Tensor
+    slot_row: torch.Tensor
+    num_experts: int | None = None
+
+
+def _local_experts(experts, num_experts: int) -> tuple[int, int]:
+    begin, count = (0, num_experts) if experts is None else experts
+    _need(0 <= begin and 0 < count and begin + count <= num_experts, "experts must be a (begin, count) range of them")
+    return begin, count
+
+
+def _plan_buffers(T: int, k: int, count: int, dev: torch.device, with_ids: bool):
+    """One allocation: [weights | ids |] row_token | slot_row | offsets | scratch, in int32 words."""
+    R = T * k
+    scratch = _native.lib().bs_fp8_moe_scratch_bytes(T, count) // 4
+    head = 2 * R if with_ids else 0
+    buf = torch.empty(head + 2 * R + count + 1 + scratch, dtype=torch.int32, device=dev)
+    row_token, slot_row = buf[head:head + R], buf[head + R:head + 2 * R].view(T, k)
+    at = head + 2 * R
+    return buf, row_token, slot_row, buf[at:at + count + 1], buf.data_ptr() + 4 * (at + count + 1), 4 * scratch
+
+
+def moe_route(logits: torch.Tensor, top_k: int, *, renormalize: bool = True, scale: float = 1.0,
+              experts: tuple[int, int] | None = None) -> MoeRoute:
+    """Router of a mixture of experts: logits [T, E] (bf16 or fp32) -> the top_k experts of each token (largest
+    logits, equal ones by lower index), their weights scale * softmax (over the chosen, or over all experts with
+    renormalize=False), and the dispatch plan for the local experts (begin, count) (None: all). Logits of -inf
+    or NaN are never chosen; slots left over have id -1 and weight 0."""
+    _need(logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32), "logits must be bf16 or fp32 [T, E]")
+    dev = _cuda(logits)
+    T, E = logits.shape
+    _need(0 < E <= MAX_EXPERTS, f"1 to {MAX_EXPERTS} experts are supported")
+    _need(0 < top_k <= min(E, MAX_TOP_K), f"top_k must be 1 to {MAX_TOP_K} and at most the number of experts")
+    begin, count = _local_experts(experts, E)
+    if logits.stride(1) != 1 or (T > 1 and logits.stride(0) < E):
+        logits = logits.contiguous()
+    with _native.device_guard(dev):
+        buf, row_token, slot_row, offsets, scratch, scratch_bytes = _plan_buffers(T, top_k, count, dev, True)
+        R = T * top_k
+        weights, ids = buf[:R].view(torch.float32).view(T, top_k), buf[R:2 * R].view(T, top_k)
+        base = buf.data_ptr()
+        _native.check(_native.lib().bs_fp8_moe_route(
+            logits.data_ptr(), int(logits.dtype == torch.float32), max(E, logits.stride(0)), T, E, top_k,
+            int(renormalize), float(scale), begin, count, base, base + 4 * R, offsets.data_ptr(), base + 8 * R,
+            base + 12 * R, scratch, scratch_bytes, _native.stream_handle(dev)), "bs_fp8_moe_route")
+    return MoeRoute(weights, ids, offsets, row_token, slot_row, E)
+
+
+def moe_dispatch(ids: torch.Tensor, weights: torch.Tensor | None, num_experts: int, *,
+                 experts: tuple[int, int] | None = None) -> MoeRoute:
+    """The dispatch plan of a routing made elsewhere: ids int32 [T, k] (an id outside the local experts, such as
+    -1, has no row), weights fp32 [T, k] (None if no weighted sum follows)."""
+    _need(ids.dim() == 2 and ids.dtype == torch.int32, "ids must be int32 [T, k]")
+    dev = _cuda(ids) if weights is None else _cuda(ids, weights)
+    _need(weights is None or (weights.dtype == torch.float32 and weights.shape == ids.shape), "weights must be fp32 like ids")
+    T, k = ids.shape
+    _need(0 < num_experts <= MAX_EXPERTS, f"1 to {MAX_EXPERTS} experts are supported")
+    _need(0 < k <= MAX_TOP_K, f"1 to {MAX_TOP_K} slots per token are supported")
+    begin, count = _local_experts(experts, num_experts)
+    ids = ids.contiguous()
+    with _native.device_guard(dev):
+        buf, row_token, slot_row, offsets, scratch, scratch_bytes = _plan_buffers(T, k, count, dev, False)
+        _native.check(_native.lib().bs_fp8_moe_dispatch(
+            ids.data_ptr(), T, num_experts, k, begin, count, offsets.data_ptr(), row_token.data_ptr(),
+            slot_row.data_ptr(), scratch, scratch_bytes, _native.stream_handle(dev)), "bs_fp8_moe_dispatch")
+    return MoeRoute(None if weights is None else weights.contiguous(), ids, offsets, row_token, slot_row, num_experts)
+
+
+def _check_grouped(A, B, As, Bs, route: MoeRoute, b_tiled: bool):
+    """Checks and geometry of a grouped product: (device, A, As, Bs, rows of A, R, rows expected, E, N, K)."""
+    _need(A.dim() == 2 and A.dtype in (E4M3, torch.uint8), "A must be e4m3 [rows, K]")
+    _need(B.dtype in (E4M3, torch.uint8) and B.is_contiguous(), "weights must be contiguous e4m3")
+    if b_tiled:
+        _need(B.dim() == 5 and tuple(B.shape[3:]) == (BLOCK, BLOCK),
+              "tile-first weights must be [E, N/128, K/128, 128, 128] bytes")
+        E, N, K = B.shape[0], B.shape[1] * BLOCK, B.shape[2] * BLOCK
+    else:
+        _need(B.dim() == 3, "row-major weights must be e4m3 [E, N, K]")
+        E, N, K = B.shape
+        _need(N % BLOCK == 0 and K % BLOCK == 0, "N and K must be multiples of 128")
+    off, rt = route.offsets, route.row_token
+    dev = _cuda(A, B, As, Bs, off, rt)
+    _need(off.dtype == torch.int32 and rt.dtype == torch.int32 and off.is_contiguous() and rt.is_contiguous(),
+          "the route's plan must be contiguous int32")
+    _need(0 < E <= MAX_EXPERTS and off.shape == (E + 1,), f"the route has {off.numel() - 1} local experts, the weights {E}")
+    _need(A.shape[1] == K, f"A has K={A.shape[1]}, weights have K={K}")
+    _need(As.dtype == torch.float32 and Bs.dtype == torch.float32, "scales must be fp32")
+    _need(As.shape == (A.shape[0], K // BLOCK), "As must be [rows, K/128]")
+    _need(Bs.shape == (E, N // BLOCK, K // BLOCK), "Bs must be [E, N/128, K/128]")
+    if not A.is_contiguous():
+        A = A.contiguous()
+    R = rt.numel()
+    hint = R if not route.num_experts else -(-R * E // route.num_experts)
+    return dev, A, As.contiguous(), Bs.contiguous(), A.shape[0], R, min(hint, R), E, N, K
+
+
+def grouped_gemm(A: torch.Tensor, B: torch.Tensor, As: torch.Tensor, Bs: torch.Tensor, route: MoeRoute, *,
+                 b_tiled: bool = False, gather: bool = False, out: torch.Tensor | None = None,
+                 out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """Block-scaled FP8 product of each row with its expert's weights: C[r] = gemm(A[r], B[e]) for the rows r of
+    expert e in `route`, bf16 or fp32 [T * k, N]. A holds the rows themselves (e.g. grouped_gemm_silu_quant's Q), or
+    with gather=True the tokens. Rows past route.offsets[-1] are not written."""
+    dev, A, As, Bs, rows_a, R, hint, E, N, K = _check_grouped(A, B, As, Bs, route, b_tiled)
+    _need(gather or rows_a >= R, f"A has {rows_a} rows, the route has {R}")
+    if out is None:
+        out = torch.empty((R, N), dtype=out_dtype, device=dev)
+    _need(out.dtype in (torch.bfloat16, torch.float32), "output must be bf16 or fp32")
+    _need(out.device == dev and out.shape == (R, N) and out.stride(1) == 1, "output must be [T * k, N] with contiguous rows")
+    with _native.device_guard(dev):
+        _native.check(_native.lib().bs_fp8_grouped_gemm(
+            A.data_ptr(), B.data_ptr(), out.data_ptr(), As.data_ptr(), Bs.data_ptr(), route.offsets.data_ptr(),
+            route.row_token.data_ptr() if gather else None, rows_a, R, hint, E, N, K, out.stride(0) if R > 1 else N,
+            int(b_tiled), int(out.dtype == torch.float32), _native.stream_handle(dev)), "bs_fp8_grouped_gemm")
+    return out
+
+
+def grouped_gemm_silu_quant(A: torch.Tensor, B: torch.Tensor, As: torch.Tensor, Bs: torch.Tensor, route: MoeRoute, *,
+                            b_tiled: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """gemm_silu_quant of each row's token with its expert's [gate; up] weights: A e4m3 [T, K] holds the tokens, read
+    in place through route.row_token. Returns Q e4m3 [T * k, I] and Qs fp32 [T * k, I/128] in row order; rows
+    past route.offsets[-1] are not written."""
+    dev, A, As, Bs, rows_a, R, hint, E, N2, K = _check_grouped(A, B, As, Bs, route, b_tiled)
+    _need(N2 % (2 * BLOCK) == 0, "gate_up rows must be a multiple of 256")
+    inter = N2 // 2
+    Q = torch.empty((R, inter), dtype=E4M3, device=dev)
+    Qs = torch.empty((R, inter // BLOCK), dtype=torch.float32, device=dev)
+    with _native.device_guard(dev):
+        _native.check(_native.lib().bs_fp8_grouped_gemm_silu_quant(
+            A.data_ptr(), B.data_ptr(), Q.data_ptr(), As.data_ptr(), Bs.data_ptr(), Qs.data_ptr(),
+            route.offsets.data_ptr(), route.row_token.data_ptr(), rows_a, R, hint, E, N2, K, int(b_tiled),
+            _native.stream_handle(dev)), "bs_fp8_grouped_gemm_silu_quant")
+    return Q, Qs
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """t with contiguous rows that start on 16 bytes (a copy where they do not)."""
+    per16 = 16 // t.element_size()
+    if t.stride(-1) != 1 or (t.shape[0] > 1 and (t.stride(0) % per16 or t.stride(0) < t.shape[1])) or t.data_ptr() % 16:
+        return t.contiguous()
+    return t
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def block_norm_quant(y: torch.Tensor, residual: torch.Tensor, *, post_weight: torch.Tensor | None = None,
+                     gate: torch.Tensor | None = None, scale: float = 1.0, residual_scale: float = 1.0,
+                     pre_weight: torch.Tensor | None = None, eps: float = 1e-6, route: MoeRoute | None = None,
+                     out: torch.Tensor | None = None):
+    """The end of a block and the start of the next one, in one pass and in fp32:
+      z = y, or with `route` the experts' rows summed per token, sum_s weights[t, s] * y[slot_row[t, s]]
+      n = rmsnorm(z) * post_weight                     (post_weight None: n = z)
+      h = residual_scale * residual + scale * gate * n
+      A, As = group_quant(rmsnorm(h) * pre_weight)     (pre_weight None: not made)
+    y bf16 [T, H] (or [rows, H] with `route`), residual bf16 or fp32 [T, H], gate bf16 [H], [T, 1] or [T, H]. h is
+    rounded once, into `out` (a new tensor like residual; pass out=residual to update it in place); A is
+    taken from the unrounded h. Returns (h, A e4m3 [T, H], As fp32 [T, H/128]), or h alone without pre_weight."""
+    bf16 = torch.bfloat16
+    _need(y.dim() == 2 and y.dtype == bf16, "y must be bf16 [rows, H]")
+    _need(residual.dim() == 2 and residual.dtype in (bf16, torch.float32), "residual must be bf16 or fp32 [T, H]")
+    dev = _cuda(y, residual)
+    T, H = residual.shape
+    _need(H % BLOCK == 0 and 0 < H <= 16384, "H must be a multiple of 128, at most 16384")
+    _need(y.shape[1] == H and (route is not None or y.shape[0] == T), "y must have residual's shape (or be a route's rows)")
+    y, residual = _rows16(y), _rows16(residual)
+    for w in (post_weight, pre_weight):
+        _need(w is None or (w.shape == (H,) and w.dtype == bf16 and w.device == dev and w.is_contiguous()
+                            and w.data_ptr() % 16 == 0), "norm weights must be contiguous bf16 [H] on the same device")
+    kind, ldg = 0, 0
+    if gate is not None:
+        _need(gate.dtype == bf16 and gate.device == dev, "gate must be bf16 on the same device")
+        if gate.dim() == 1:
+            _need(gate.shape == (H,), "gate must be [H], [T, 1] or [T, H]")
+            kind, gate = 1, gate.contiguous()
+            if gate.data_ptr() % 16:
+                gate = gate.clone()
+        else:
+            _need(gate.dim() == 2 and gate.shape[0] == T and gate.shape[1] in (1, H), "gate must be [H], [T, 1] or [T, H]")
+            if gate.shape[1] == 1:
+                if T > 1 and gate.stride(0) < 1:
+                    gate = gate.contiguous()
+                kind, ldg = 2, gate.stride(0) if T > 1 else 1
+            else:
+                gate = _rows16(gate)
+                kind, ldg = 3, _row_stride(gate)
+    w_ptr = s_ptr = None
+    k = 0
+    if route is not None:
+        _need(route.weights is not None and route.weights.shape == route.slot_row.shape, "the route has no weights")
+        _cuda(y, route.weights, route.slot_row)
+        _need(route.weights.dtype == torch.float32 and route.weights.is_contiguous()
+              and route.slot_row.dtype == torch.int32 and route.slot_row.is_contiguous(),
+              "the route's weights and rows must be contiguous fp32 and int32")
+        _need(route.slot_row.shape[0] == T, f"the route has {route.slot_row.shape[0]} tokens, the residual {T}")
+        w_ptr, s_ptr, k = route.weights.data_ptr(), route.slot_row.data_ptr(), route.slot_row.shape[1]
+    if out is None:
+        out = torch.empty((T, H), dtype=residual.dtype, device=dev)
+    _need(out.shape == (T, H) and out.dtype == residual.dtype and out.device == dev and _rows16(out) is out,
+          "out must be like residual, with contiguous 16-byte aligned rows")
+    A = As = None
+    if pre_weight is not None:
+        A = torch.empty((T, H), dtype=E4M3, device=dev)
+        As = torch.empty((T, H // BLOCK), dtype=torch.float32, device=dev)
+    with _native.device_guard(dev):
+        _native.check(_native.lib().bs_fp8_block_norm_quant(
+            y.data_ptr(), _row_stride(y), y.shape[0], w_ptr, s_ptr, k, residual.data_ptr(), _row_stride(residual),
+            out.data_ptr(), _row_stride(out), int(residual.dtype == torch.float32), _native.ptr(post_weight),
+            _native.ptr(gate), kind, ldg, float(scale), float(residual_scale), _native.ptr(pre_weight), float(eps),
+            _native.ptr(A), _native.ptr(As), T, H, _native.stream_handle(dev)), "bs_fp8_block_norm_quant")
+    return out if pre_weight is None else (out, A, As)
