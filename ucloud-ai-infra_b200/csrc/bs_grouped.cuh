@@ -28,6 +28,7 @@ struct GroupedParams {
   int b_tiled, out_f32;
   const int* offsets;   // [E + 1]
   const int* row_token; // [R]: row of A for each row; nullptr: the row itself
+  const uint8_t* A;     // [rows_a, K]
   const float* As;      // [rows_a, KB]
   const float* Bs;      // [E, nblk, KB]
   void* out;            // plain: [R, ldc]; fused: Q [R, I]
@@ -121,9 +122,22 @@ __device__ __forceinline__ int source_row(const GroupedParams& p, int r) {
   return static_cast<unsigned>(t) < static_cast<unsigned>(p.rows_a) ? t : 0;
 }
 
+// 16 bytes from global to shared memory, not through L1, tracked by the thread's cp.async groups.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// One arrival on `bar` when every copy this thread has issued so far has landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // ---------------------------------------------------------------- many rows per expert
-// Roles, stages, TMEM buffers and the promotion are those of k_prefill (bs_prefill.cuh); the producer is a whole warp
-// when the rows are gathered: lane l brings rows 4l..4l+3 of the tile with one gathering load per K block.
+// Roles, stages, TMEM buffers and the promotion are those of k_prefill (bs_prefill.cuh). When the rows are gathered,
+// warps 10 and 11 bring them, 64 rows each, with 16-byte cp.async copies written where the 128-byte swizzle of a TMA
+// load would put them (chunk c of row r at chunk c ^ (r % 8)). A gathering TMA load (four rows each) was measured first
+// and is the bound of the kernel there: 8192 tokens x 8 of 64 experts, K = 5120, N = 2048, one product: 1894 us gathered
+// by TMA, 843 us with the rows already in order.
 template <bool FUSED>
 struct GroupedRowsCfg {
   using Regs = RegSplit<384, 168, 40, 232>;
@@ -132,8 +146,9 @@ struct GroupedRowsCfg {
   static constexpr int kABytes = 128 * 128;
   static constexpr int kStageBytes = kABytes + 256 * 128;
   static constexpr int kXchOff = kStages * kStageBytes;
-  static constexpr int kXchBytes = FUSED ? 128 * 2 * 4 : 0;
-  static constexpr int kBarOff = kXchOff + kXchBytes;
+  static constexpr int kXchBytes = FUSED ? 128 * 2 * 4 : 8 * 2048;  // amax halves; plain: 2 KB per promotion warp
+  static constexpr int kTokOff = kXchOff + kXchBytes;               // gathered rows of the loaders' tile
+  static constexpr int kBarOff = kTokOff + 128 * 4;
   static constexpr int kTableOff = kBarOff + 256;
   static constexpr int kSmemBytes = kTableOff + static_cast<int>(sizeof(GroupTable)) + 1024;
   static constexpr int kTmemCols = 512;
@@ -155,13 +170,15 @@ __global__ void __launch_bounds__(GroupedRowsCfg<FUSED>::kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* amax_x = reinterpret_cast<float*>(smem + Cfg::kXchOff);  // fused: [128 rows][2 halves]
+  int* tok = reinterpret_cast<int*>(smem + Cfg::kTokOff);
+  const bool gather = p.row_token != nullptr;
   GroupTable& table = *reinterpret_cast<GroupTable*>(smem + Cfg::kTableOff);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
-      mbar_init(&full[i], 1);
+      mbar_init(&full[i], gather ? 1 + 64 : 1);  // the producer, and the loader threads
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -192,44 +209,32 @@ __global__ void __launch_bounds__(GroupedRowsCfg<FUSED>::kThreads, 1)
 
   if (warp >= 8) {
     regs_decrease<Cfg::Regs::kProducer>();
-    if (warp == 8) {
+    if (warp == 8 && lane == 0) {
       // ------------------------------------------------------------ TMA producer
       const uint64_t pol_a = policy_evict_last(), pol_b = policy_evict_normal();
-      const bool gather = p.row_token != nullptr;
       int s = 0;
       uint32_t ph = 0, issued = 0, parity_bits = 0;
       bool ok = true;
       for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
         const GroupTile t = find_tile(table, tile, 128);
-        int4 rows = make_int4(0, 0, 0, 0);
-        if (gather) {
-          const int last = t.row + t.rows - 1, r = t.row + 4 * lane;
-          rows = make_int4(source_row(p, min(r, last)), source_row(p, min(r + 1, last)),
-                           source_row(p, min(r + 2, last)), source_row(p, min(r + 3, last)));
-        }
         const int nb = t.expert * nblk;
         for (int kb = 0; kb < KB; ++kb) {
-          if (lane == 0) ok = mbar_wait(&empty[s], ph ^ 1, abort_flag, p.status, kErrTimeoutEmpty);
-          ok = __shfl_sync(0xffffffffu, ok, 0);
+          ok = mbar_wait(&empty[s], ph ^ 1, abort_flag, p.status, kErrTimeoutEmpty);
           if (!ok) break;
           uint8_t* st = smem + s * Cfg::kStageBytes;
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&full[s], Cfg::kStageBytes);
-            if constexpr (FUSED) {
+          mbar_arrive_expect_tx(&full[s], gather ? Cfg::kStageBytes - Cfg::kABytes : Cfg::kStageBytes);
+          if constexpr (FUSED) {
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                load_weight_half(st + Cfg::kABytes + 16384 * h, &tmB, &full[s], nb + t.tn, h, kb, KB, p.b_tiled, pol_b);
-                load_weight_half(st + Cfg::kABytes + 16384 * h + 8192, &tmB, &full[s], nb + t.tn + I_blk, h, kb, KB,
-                                 p.b_tiled, pol_b);
-              }
-            } else {
-              load_weight_box(st + Cfg::kABytes, &tmB, &full[s], nb + 2 * t.tn, kb, KB, p.b_tiled, pol_b);
-              load_weight_box(st + Cfg::kABytes + 16384, &tmB, &full[s], nb + 2 * t.tn + 1, kb, KB, p.b_tiled, pol_b);
+            for (int h = 0; h < 2; ++h) {
+              load_weight_half(st + Cfg::kABytes + 16384 * h, &tmB, &full[s], nb + t.tn, h, kb, KB, p.b_tiled, pol_b);
+              load_weight_half(st + Cfg::kABytes + 16384 * h + 8192, &tmB, &full[s], nb + t.tn + I_blk, h, kb, KB,
+                               p.b_tiled, pol_b);
             }
-            if (!gather) tma_load_2d(st, &tmA, &full[s], kb * 128, t.row, pol_a);
+          } else {
+            load_weight_box(st + Cfg::kABytes, &tmB, &full[s], nb + 2 * t.tn, kb, KB, p.b_tiled, pol_b);
+            load_weight_box(st + Cfg::kABytes + 16384, &tmB, &full[s], nb + 2 * t.tn + 1, kb, KB, p.b_tiled, pol_b);
           }
-          __syncwarp();
-          if (gather) tma_gather4(st + 512 * lane, &tmA, &full[s], kb * 128, rows, pol_a);
+          if (!gather) tma_load_2d(st, &tmA, &full[s], kb * 128, t.row, pol_a);
           issued |= 1u << s;
           parity_bits = (parity_bits & ~(1u << s)) | (ph << s);
           if (++s == S) {
@@ -238,10 +243,56 @@ __global__ void __launch_bounds__(GroupedRowsCfg<FUSED>::kThreads, 1)
           }
         }
       }
-      if (!ok && lane == 0)  // leave no copy in flight
-        for (int i = 0; i < S; ++i)
+      if (!ok) {
+        // Leave no copy in flight. (With loaders the barrier also waits for them, and one that gave up never
+        // arrives: the copies land within microseconds.)
+        if (gather) pause_ns(2000000ull);
+        for (int i = 0; i < S && !gather; ++i)
           if (issued & (1u << i))
             mbar_wait(&full[i], (parity_bits >> i) & 1u, abort_flag, p.status, kErrTimeoutDrain, 100000000ull);
+      }
+    } else if (warp >= 10 && gather) {
+      // ------------------------------------------------------------ row loaders
+      // Copy i of a lane: chunk lane % 8 of row 64 w + 4 i + lane / 8. The stage's barrier hears from every loader thread
+      // when its copies have landed; the MMA issuer makes them visible to the tensor core (its fence), so a loader
+      // never waits for its own copies.
+      const int w = warp - 10, c = lane & 7, sub = lane >> 3;
+      int* mine = tok + 64 * w;
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      auto sources = [&](int tile, int& a, int& b) {  // of rows lane and lane + 32 of this warp's 64
+        if (tile >= num_tiles) return;
+        const GroupTile t = find_tile(table, tile, 128);
+        a = source_row(p, t.row + min(64 * w + lane, t.rows - 1));
+        b = source_row(p, t.row + min(64 * w + lane + 32, t.rows - 1));
+      };
+      int src0 = 0, src1 = 0;
+      sources(blockIdx.x, src0, src1);
+      for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
+        __syncwarp();
+        mine[lane] = src0;
+        mine[lane + 32] = src1;
+        __syncwarp();
+        sources(tile + gridDim.x, src0, src1);  // the next tile's, a whole tile ahead
+        for (int kb = 0; kb < KB; ++kb) {
+          ok = mbar_wait_warp(&empty[s], ph ^ 1, abort_flag, p.status, kErrTimeoutEmpty);
+          if (!ok) break;
+          const uint32_t st = smem_u32(smem + s * Cfg::kStageBytes) + 8192 * w;
+          const uint8_t* src = p.A + static_cast<size_t>(kb) * 128 + c * 16;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int r = 4 * i + sub;
+            cp_async16(st + 128 * r + 16 * (c ^ (r & 7)), src + static_cast<size_t>(mine[r]) * (static_cast<size_t>(KB) * 128));
+          }
+          cp_async_arrive(&full[s]);
+          if (++s == S) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+      cp_async_wait_all();
     } else if (warp == 9 && lane == 0) {
       // ------------------------------------------------------------ MMA issuer
       constexpr uint32_t idesc = idesc_e4m3_f32(128, 256);
@@ -253,6 +304,7 @@ __global__ void __launch_bounds__(GroupedRowsCfg<FUSED>::kThreads, 1)
           ok = mbar_wait(&full[s], ph, abort_flag, p.status, kErrTimeoutFull) &&
                mbar_wait(&pempty[b], pph ^ 1, abort_flag, p.status, kErrTimeoutPEmpty);
           if (!ok) break;
+          if (gather) fence_proxy_async_smem();  // the loaders' rows, written by ordinary copies
           tc_fence_after();
           const uint32_t a0 = smem_u32(smem + s * Cfg::kStageBytes);
           const uint32_t b0 = a0 + Cfg::kABytes;
@@ -285,13 +337,20 @@ __global__ void __launch_bounds__(GroupedRowsCfg<FUSED>::kThreads, 1)
     int b = 0;
     uint32_t pph = 0;
     bool ok = true;
+    auto source_of = [&](int tile) {
+      if (tile >= num_tiles) return 0;
+      const GroupTile t = find_tile(table, tile, 128);
+      return source_row(p, t.row + (r < t.rows ? r : 0));
+    };
+    int src = source_of(blockIdx.x);
     for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x) {
       const GroupTile t = find_tile(table, tile, 128);
       const bool row_ok = r < t.rows;
       const int row = t.row + (row_ok ? r : 0);
       const int nb = FUSED ? t.tn : 2 * t.tn + wg;  // block inside the expert; fused: the gate's
       const bool col_ok = nb < nblk;
-      const float* as_row = p.As + static_cast<size_t>(source_row(p, row)) * KB;
+      const float* as_row = p.As + static_cast<size_t>(src) * KB;
+      src = source_of(tile + gridDim.x);  // a whole tile ahead
       const float* bs_row = p.Bs + (static_cast<size_t>(t.expert) * nblk + (col_ok ? nb : 0)) * KB;
       const float* bu_row = bs_row + static_cast<size_t>(FUSED ? I_blk : 0) * KB;
 
@@ -369,21 +428,40 @@ __global__ void __launch_bounds__(GroupedRowsCfg<FUSED>::kThreads, 1)
       }
 
       if constexpr (!FUSED) {
-        if (ok && row_ok && col_ok) {
-          const size_t at = static_cast<size_t>(row) * p.ldc + static_cast<size_t>(nb) * 128;
+        if (ok && col_ok) {
           if (p.out_f32) {
-            float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+            if (row_ok) {
+              float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + static_cast<size_t>(row) * p.ldc +
+                                                      static_cast<size_t>(nb) * 128);
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              dst[j] = make_float4(lo_f(acc[2 * j]), hi_f(acc[2 * j]), lo_f(acc[2 * j + 1]), hi_f(acc[2 * j + 1]));
+              for (int j = 0; j < 32; ++j)
+                dst[j] = make_float4(lo_f(acc[2 * j]), hi_f(acc[2 * j]), lo_f(acc[2 * j + 1]), hi_f(acc[2 * j + 1]));
+            }
           } else {
-            uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + at);
+            // A warp's 32 rows x 32 columns at a time through 2 KB of shared memory (chunks of 16 bytes, swizzled), so
+            // that a store writes whole 64-byte pieces of eight rows instead of 16 bytes of 32 rows.
+            uint4* buf = reinterpret_cast<uint4*>(smem + Cfg::kXchOff) + warp * 128;
+            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + static_cast<size_t>(t.row + q * 32) * p.ldc +
+                                 static_cast<size_t>(nb) * 128 + (lane & 3) * 8;
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              dst[j] = make_uint4(pack_bf16x2(lo_f(acc[4 * j]), hi_f(acc[4 * j])),
-                                  pack_bf16x2(lo_f(acc[4 * j + 1]), hi_f(acc[4 * j + 1])),
-                                  pack_bf16x2(lo_f(acc[4 * j + 2]), hi_f(acc[4 * j + 2])),
-                                  pack_bf16x2(lo_f(acc[4 * j + 3]), hi_f(acc[4 * j + 3])));
+            for (int h = 0; h < 4; ++h) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const int j = 16 * h + 4 * c;  // columns 2j .. 2j + 7
+                buf[lane * 4 + (c ^ ((lane >> 1) & 3))] =
+                    make_uint4(pack_bf16x2(lo_f(acc[j]), hi_f(acc[j])), pack_bf16x2(lo_f(acc[j + 1]), hi_f(acc[j + 1])),
+                               pack_bf16x2(lo_f(acc[j + 2]), hi_f(acc[j + 2])),
+                               pack_bf16x2(lo_f(acc[j + 3]), hi_f(acc[j + 3])));
+              }
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int rr = 8 * i + (lane >> 2);
+                const uint4 v = buf[rr * 4 + ((lane & 3) ^ ((rr >> 1) & 3))];
+                if (q * 32 + rr < t.rows) *reinterpret_cast<uint4*>(dst + static_cast<size_t>(rr) * p.ldc + 32 * h) = v;
+              }
+              __syncwarp();
+            }
           }
         }
       } else {

@@ -109,7 +109,7 @@ int validate_grouped(const void* A, const void* B, const void* out, const float*
   return BS_OK;
 }
 
-bs::GroupedParams grouped_params(const float* As, const float* Bs, const int* offsets, const int* row_token, int rows_a,
+bs::GroupedParams grouped_params(const void* A, const float* As, const float* Bs, const int* offsets, const int* row_token, int rows_a,
                                  int R, int E, int N, int K, int b_tiled, int* status) {
   bs::GroupedParams p = {};
   p.E = E;
@@ -120,6 +120,7 @@ bs::GroupedParams grouped_params(const float* As, const float* Bs, const int* of
   p.b_tiled = b_tiled;
   p.offsets = offsets;
   p.row_token = row_token;
+  p.A = static_cast<const uint8_t*>(A);
   p.As = As;
   p.Bs = Bs;
   p.status = status;
@@ -196,7 +197,7 @@ int bs_fp8_grouped_gemm(const void* A, const void* B, void* C, const float* As, 
   if (rc != BS_OK || R == 0) return rc;
   DeviceState* d = device_state();
   if (!d) return BS_ERR_CUDA;
-  bs::GroupedParams p = grouped_params(As, Bs, offsets, row_token, rows_a, R, E, N, K, b_tiled, d->status);
+  bs::GroupedParams p = grouped_params(A, As, Bs, offsets, row_token, rows_a, R, E, N, K, b_tiled, d->status);
   p.ldc = ldc;
   p.out_f32 = out_dtype;
   p.out = C;
@@ -211,7 +212,7 @@ int bs_fp8_grouped_gemm_silu_quant(const void* A, const void* B, void* Q, const 
   if (rc != BS_OK || R == 0) return rc;
   DeviceState* d = device_state();
   if (!d) return BS_ERR_CUDA;
-  bs::GroupedParams p = grouped_params(As, Bs, offsets, row_token, rows_a, R, E, N2, K, b_tiled, d->status);
+  bs::GroupedParams p = grouped_params(A, As, Bs, offsets, row_token, rows_a, R, E, N2, K, b_tiled, d->status);
   p.ldc = N2 / 2;
   p.out = Q;
   p.qs = Qs;
