@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(GroupedRowsCfg<FUSED>::kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* amax_x = reinterpret_cast<float*>(smem + Cfg::kXchOff);  // fused: [128 rows][2 halves]
-  int* tok = reinterpret_cast<int*>(smem + Cfg::kTokOff);
+  uint32_t* tok = reinterpret_cast<uint32_t*>(smem + Cfg::kTokOff);
   const bool gather = p.row_token != nullptr;
   GroupTable& table = *reinterpret_cast<GroupTable*>(smem + Cfg::kTableOff);
 
@@ -257,33 +257,40 @@ __global__ void __launch_bounds__(GroupedRowsCfg<FUSED>::kThreads, 1)
       // when its copies have landed; the MMA issuer makes them visible to the tensor core (its fence), so a loader
       // never waits for its own copies.
       const int w = warp - 10, c = lane & 7, sub = lane >> 3;
-      int* mine = tok + 64 * w;
+      uint32_t* mine = tok + 64 * w;  // start of row 4 i + sub in 16-byte units, at [16 sub + i]
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
-      auto sources = [&](int tile, int& a, int& b) {  // of rows lane and lane + 32 of this warp's 64
+      const uint32_t row16 = static_cast<uint32_t>(KB) * 8;
+      // of the rows at mine[lane] and mine[lane + 32]
+      auto sources = [&](int tile, uint32_t& a, uint32_t& b) {
         if (tile >= num_tiles) return;
         const GroupTile t = find_tile(table, tile, 128);
-        a = source_row(p, t.row + min(64 * w + lane, t.rows - 1));
-        b = source_row(p, t.row + min(64 * w + lane + 32, t.rows - 1));
+        const int ra = 64 * w + 4 * (lane & 15) + (lane >> 4);
+        a = static_cast<uint32_t>(source_row(p, t.row + min(ra, t.rows - 1))) * row16;
+        b = static_cast<uint32_t>(source_row(p, t.row + min(ra + 2, t.rows - 1))) * row16;
       };
-      int src0 = 0, src1 = 0;
+      uint32_t src0 = 0, src1 = 0;
       sources(blockIdx.x, src0, src1);
+      const uint32_t even = 128 * sub + 16 * (c ^ sub), odd = 128 * sub + 16 * (c ^ (sub + 4));  // rows 8 j + sub, + 4
       for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
         __syncwarp();
         mine[lane] = src0;
         mine[lane + 32] = src1;
         __syncwarp();
         sources(tile + gridDim.x, src0, src1);  // the next tile's, a whole tile ahead
-        for (int kb = 0; kb < KB; ++kb) {
+        const uint8_t* src = p.A + c * 16;
+        for (int kb = 0; kb < KB; ++kb, src += 128) {
           ok = mbar_wait_warp(&empty[s], ph ^ 1, abort_flag, p.status, kErrTimeoutEmpty);
           if (!ok) break;
           const uint32_t st = smem_u32(smem + s * Cfg::kStageBytes) + 8192 * w;
-          const uint8_t* src = p.A + static_cast<size_t>(kb) * 128 + c * 16;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int r = 4 * i + sub;
-            cp_async16(st + 128 * r + 16 * (c ^ (r & 7)), src + static_cast<size_t>(mine[r]) * (static_cast<size_t>(KB) * 128));
+          for (int i = 0; i < 16; i += 4) {
+            const uint4 o = *reinterpret_cast<const uint4*>(mine + 16 * sub + i);
+            cp_async16(st + even + 512 * i, src + static_cast<uint64_t>(o.x) * 16);
+            cp_async16(st + odd + 512 * (i + 1), src + static_cast<uint64_t>(o.y) * 16);
+            cp_async16(st + even + 512 * (i + 2), src + static_cast<uint64_t>(o.z) * 16);
+            cp_async16(st + odd + 512 * (i + 3), src + static_cast<uint64_t>(o.w) * 16);
           }
           cp_async_arrive(&full[s]);
           if (++s == S) {

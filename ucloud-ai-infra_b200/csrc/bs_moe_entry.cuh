@@ -105,6 +105,7 @@ int validate_grouped(const void* A, const void* B, const void* out, const float*
   if (!offsets || rows_a == 0 || (!row_token && rows_a < R)) return BS_ERR_ARG;
   // 32-bit tile counts and TMA coordinates
   if (static_cast<long long>(E) * N * (b_tiled ? K / 128 : 1) >= (1ll << 31)) return BS_ERR_ARG;
+  if (static_cast<long long>(rows_a) * (K / 16) >= (1ll << 32)) return BS_ERR_ARG;
   if ((static_cast<long long>(R) / 16 + E) * (N / 128) >= (1ll << 31)) return BS_ERR_ARG;
   return BS_OK;
 }
