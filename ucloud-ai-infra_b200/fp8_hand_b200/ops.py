@@ -17,6 +17,7 @@ E4M3 = torch.float8_e4m3fn
 BLOCK = 128
 MAX_EXPERTS = 512
 MAX_TOP_K = 32
+_BYTES = (E4M3, torch.uint8)
 
 
 def _need(cond: bool, msg: str) -> None:
@@ -235,12 +236,14 @@ def gemm_silu_quant(A: torch.Tensor, B: torch.Tensor, As: torch.Tensor, Bs: torc
 
 
 # ------------------------------------------------------------------ mixture of experts
+# At decode sizes the kernels of these operators take a few microseconds, so the checks below are written for the
+# host's time: no message is built and no view is made unless it is needed.
 @dataclass(slots=True)
 class MoeRoute:
     """A routed batch of T tokens with k slots each (moe_route, moe_dispatch), all on the device. Rows are the
     (token, slot) pairs whose expert is local, sorted by expert and then by place in ids.
 
-      weights    fp32 [T, k]           weight of each slot
+      weights    fp32 [T, k]           weight of each slot (None: not known)
       ids        int32 [T, k]          expert of each slot, -1 for none
       offsets    int32 [experts + 1]   rows of local expert e: offsets[e] .. offsets[e + 1] - 1
       row_token  int32 [T * k]         token of each row, -1 past offsets[-1]
@@ -255,21 +258,36 @@ class MoeRoute:
     num_experts: int | None = None
 
 
+def _one_device(*ts: torch.Tensor) -> int:
+    """Index of the CUDA device that holds every tensor."""
+    index = ts[0].get_device()
+    for t in ts:
+        if t.get_device() != index or index < 0 or not t.is_cuda:
+            _cuda(*ts)
+            raise ValueError("all tensors must be on the same CUDA device")
+    return index
+
+
 def _local_experts(experts, num_experts: int) -> tuple[int, int]:
-    begin, count = (0, num_experts) if experts is None else experts
+    if experts is None:
+        return 0, num_experts
+    begin, count = experts
     _need(0 <= begin and 0 < count and begin + count <= num_experts, "experts must be a (begin, count) range of them")
     return begin, count
 
 
-def _plan_buffers(T: int, k: int, count: int, dev: torch.device, with_ids: bool):
-    """One allocation: [weights | ids |] row_token | slot_row | offsets | scratch, in int32 words."""
-    R = T * k
-    scratch = _native.lib().bs_fp8_moe_scratch_bytes(T, count) // 4
-    head = 2 * R if with_ids else 0
-    buf = torch.empty(head + 2 * R + count + 1 + scratch, dtype=torch.int32, device=dev)
-    row_token, slot_row = buf[head:head + R], buf[head + R:head + 2 * R].view(T, k)
-    at = head + 2 * R
-    return buf, row_token, slot_row, buf[at:at + count + 1], buf.data_ptr() + 4 * (at + count + 1), 4 * scratch
+def _routing_limits(num_experts: int, k: int) -> None:
+    _need(0 < num_experts <= MAX_EXPERTS, f"1 to {MAX_EXPERTS} experts are supported")
+    _need(0 < k <= MAX_TOP_K, f"1 to {MAX_TOP_K} slots per token are supported")
+
+
+def _offsets_and_scratch(lib, T: int, count: int, device: torch.device):
+    """offsets [count + 1], and the address and bytes of the scratch behind it (one allocation)."""
+    scratch = lib.bs_fp8_moe_scratch_bytes(T, count)
+    if not scratch:
+        return torch.empty(count + 1, dtype=torch.int32, device=device), None, 0
+    buf = torch.empty(count + 1 + scratch // 4, dtype=torch.int32, device=device)
+    return buf[:count + 1], buf.data_ptr() + 4 * (count + 1), scratch
 
 
 def moe_route(logits: torch.Tensor, top_k: int, *, renormalize: bool = True, scale: float = 1.0,
@@ -278,72 +296,92 @@ def moe_route(logits: torch.Tensor, top_k: int, *, renormalize: bool = True, sca
     logits, equal ones by lower index), their weights scale * softmax (over the chosen, or over all experts with
     renormalize=False), and the dispatch plan for the local experts (begin, count) (None: all). Logits of -inf
     or NaN are never chosen; slots left over have id -1 and weight 0."""
-    _need(logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32), "logits must be bf16 or fp32 [T, E]")
-    dev = _cuda(logits)
+    f32 = logits.dtype == torch.float32
+    if logits.dim() != 2 or not (f32 or logits.dtype == torch.bfloat16):
+        raise ValueError("logits must be bf16 or fp32 [T, E]")
+    index = _one_device(logits)
     T, E = logits.shape
-    _need(0 < E <= MAX_EXPERTS, f"1 to {MAX_EXPERTS} experts are supported")
-    _need(0 < top_k <= min(E, MAX_TOP_K), f"top_k must be 1 to {MAX_TOP_K} and at most the number of experts")
+    if not (0 < E <= MAX_EXPERTS and 0 < top_k <= MAX_TOP_K and top_k <= E):
+        _routing_limits(E, top_k)
+        raise ValueError("top_k must be at most the number of experts")
     begin, count = _local_experts(experts, E)
-    if logits.stride(1) != 1 or (T > 1 and logits.stride(0) < E):
-        logits = logits.contiguous()
-    with _native.device_guard(dev):
-        buf, row_token, slot_row, offsets, scratch, scratch_bytes = _plan_buffers(T, top_k, count, dev, True)
-        R = T * top_k
-        weights, ids = buf[:R].view(torch.float32).view(T, top_k), buf[R:2 * R].view(T, top_k)
-        base = buf.data_ptr()
-        _native.check(_native.lib().bs_fp8_moe_route(
-            logits.data_ptr(), int(logits.dtype == torch.float32), max(E, logits.stride(0)), T, E, top_k,
-            int(renormalize), float(scale), begin, count, base, base + 4 * R, offsets.data_ptr(), base + 8 * R,
-            base + 12 * R, scratch, scratch_bytes, _native.stream_handle(dev)), "bs_fp8_moe_route")
-    return MoeRoute(weights, ids, offsets, row_token, slot_row, E)
+    ld, inner = logits.stride()
+    if inner != 1 or ld < E:
+        if inner != 1 or T > 1:
+            logits = logits.contiguous()
+        ld = E
+    lib, dev = _native.lib(), logits.device
+    weights, ids, row_token, slot_row = torch.empty((4, T, top_k), dtype=torch.int32, device=dev).unbind()
+    offsets, scratch, scratch_bytes = _offsets_and_scratch(lib, T, count, dev)
+    base, step = weights.data_ptr(), 4 * T * top_k
+    _native.call(lib.bs_fp8_moe_route, "bs_fp8_moe_route", index, logits.data_ptr(), f32, ld, T, E, top_k, renormalize,
+                 scale, begin, count, base, base + step, offsets.data_ptr(), base + 2 * step, base + 3 * step, scratch,
+                 scratch_bytes)
+    return MoeRoute(weights.view(torch.float32), ids, offsets, row_token.view(-1), slot_row, E)
 
 
 def moe_dispatch(ids: torch.Tensor, weights: torch.Tensor | None, num_experts: int, *,
                  experts: tuple[int, int] | None = None) -> MoeRoute:
     """The dispatch plan of a routing made elsewhere: ids int32 [T, k] (an id outside the local experts, such as
     -1, has no row), weights fp32 [T, k] (None if no weighted sum follows)."""
-    _need(ids.dim() == 2 and ids.dtype == torch.int32, "ids must be int32 [T, k]")
-    dev = _cuda(ids) if weights is None else _cuda(ids, weights)
-    _need(weights is None or (weights.dtype == torch.float32 and weights.shape == ids.shape), "weights must be fp32 like ids")
+    if ids.dim() != 2 or ids.dtype != torch.int32:
+        raise ValueError("ids must be int32 [T, k]")
+    if weights is not None:
+        if weights.dtype != torch.float32 or weights.shape != ids.shape:
+            raise ValueError("weights must be fp32 like ids")
+        index = _one_device(ids, weights)
+        weights = weights.contiguous()
+    else:
+        index = _one_device(ids)
     T, k = ids.shape
-    _need(0 < num_experts <= MAX_EXPERTS, f"1 to {MAX_EXPERTS} experts are supported")
-    _need(0 < k <= MAX_TOP_K, f"1 to {MAX_TOP_K} slots per token are supported")
+    _routing_limits(num_experts, k)
     begin, count = _local_experts(experts, num_experts)
     ids = ids.contiguous()
-    with _native.device_guard(dev):
-        buf, row_token, slot_row, offsets, scratch, scratch_bytes = _plan_buffers(T, k, count, dev, False)
-        _native.check(_native.lib().bs_fp8_moe_dispatch(
-            ids.data_ptr(), T, num_experts, k, begin, count, offsets.data_ptr(), row_token.data_ptr(),
-            slot_row.data_ptr(), scratch, scratch_bytes, _native.stream_handle(dev)), "bs_fp8_moe_dispatch")
-    return MoeRoute(None if weights is None else weights.contiguous(), ids, offsets, row_token, slot_row, num_experts)
+    lib, dev = _native.lib(), ids.device
+    rows = torch.empty((2, T * k), dtype=torch.int32, device=dev)
+    row_token, slot_row = rows[0], rows[1].view(T, k)
+    offsets, scratch, scratch_bytes = _offsets_and_scratch(lib, T, count, dev)
+    _native.call(lib.bs_fp8_moe_dispatch, "bs_fp8_moe_dispatch", index, ids.data_ptr(), T, num_experts, k, begin, count,
+                 offsets.data_ptr(), row_token.data_ptr(), slot_row.data_ptr(), scratch, scratch_bytes)
+    return MoeRoute(weights, ids, offsets, row_token, slot_row, num_experts)
 
 
 def _check_grouped(A, B, As, Bs, route: MoeRoute, b_tiled: bool):
-    """Checks and geometry of a grouped product: (device, A, As, Bs, rows of A, R, rows expected, E, N, K)."""
-    _need(A.dim() == 2 and A.dtype in (E4M3, torch.uint8), "A must be e4m3 [rows, K]")
-    _need(B.dtype in (E4M3, torch.uint8) and B.is_contiguous(), "weights must be contiguous e4m3")
-    if b_tiled:
-        _need(B.dim() == 5 and tuple(B.shape[3:]) == (BLOCK, BLOCK),
-              "tile-first weights must be [E, N/128, K/128, 128, 128] bytes")
-        E, N, K = B.shape[0], B.shape[1] * BLOCK, B.shape[2] * BLOCK
-    else:
-        _need(B.dim() == 3, "row-major weights must be e4m3 [E, N, K]")
-        E, N, K = B.shape
-        _need(N % BLOCK == 0 and K % BLOCK == 0, "N and K must be multiples of 128")
+    """Checks and geometry of a grouped product: (device index, A, As, Bs, rows of A, R, rows expected, E, N, K)."""
     off, rt = route.offsets, route.row_token
-    dev = _cuda(A, B, As, Bs, off, rt)
-    _need(off.dtype == torch.int32 and rt.dtype == torch.int32 and off.is_contiguous() and rt.is_contiguous(),
-          "the route's plan must be contiguous int32")
-    _need(0 < E <= MAX_EXPERTS and off.shape == (E + 1,), f"the route has {off.numel() - 1} local experts, the weights {E}")
-    _need(A.shape[1] == K, f"A has K={A.shape[1]}, weights have K={K}")
-    _need(As.dtype == torch.float32 and Bs.dtype == torch.float32, "scales must be fp32")
-    _need(As.shape == (A.shape[0], K // BLOCK), "As must be [rows, K/128]")
-    _need(Bs.shape == (E, N // BLOCK, K // BLOCK), "Bs must be [E, N/128, K/128]")
-    if not A.is_contiguous():
-        A = A.contiguous()
+    index = _one_device(A, B, As, Bs, off, rt)
+    if b_tiled:
+        if B.dim() != 5:
+            raise ValueError("tile-first weights must be [E, N/128, K/128, 128, 128] bytes")
+        E, nb, kb, r, c = B.shape
+        if r != BLOCK or c != BLOCK:
+            raise ValueError("tile-first weights must be [E, N/128, K/128, 128, 128] bytes")
+        N, K = nb * BLOCK, kb * BLOCK
+    else:
+        if B.dim() != 3:
+            raise ValueError("row-major weights must be e4m3 [E, N, K]")
+        E, N, K = B.shape
+        if N % BLOCK or K % BLOCK:
+            raise ValueError("N and K must be multiples of 128")
+        nb, kb = N // BLOCK, K // BLOCK
+    if B.dtype not in _BYTES or not B.is_contiguous():
+        raise ValueError("weights must be contiguous e4m3")
+    if A.dim() != 2 or A.dtype not in _BYTES:
+        raise ValueError("A must be e4m3 [rows, K]")
+    rows_a, ka = A.shape
+    if ka != K:
+        raise ValueError(f"A has K={ka}, weights have K={K}")
+    if As.dtype != torch.float32 or Bs.dtype != torch.float32:
+        raise ValueError("scales must be fp32")
+    if As.shape != (rows_a, kb) or Bs.shape != (E, nb, kb):
+        raise ValueError("As must be [rows, K/128] and Bs [E, N/128, K/128]")
+    if off.dtype != torch.int32 or rt.dtype != torch.int32 or not (off.is_contiguous() and rt.is_contiguous()):
+        raise ValueError("the route's plan must be contiguous int32")
+    if not 0 < E <= MAX_EXPERTS or off.numel() != E + 1:
+        raise ValueError(f"the route has {off.numel() - 1} local experts, the weights {E} (at most {MAX_EXPERTS})")
     R = rt.numel()
-    hint = R if not route.num_experts else -(-R * E // route.num_experts)
-    return dev, A, As.contiguous(), Bs.contiguous(), A.shape[0], R, min(hint, R), E, N, K
+    hint = min(R, -(-R * E // route.num_experts)) if route.num_experts else R
+    return index, A.contiguous(), As.contiguous(), Bs.contiguous(), rows_a, R, hint, E, N, K
 
 
 def grouped_gemm(A: torch.Tensor, B: torch.Tensor, As: torch.Tensor, Bs: torch.Tensor, route: MoeRoute, *,
@@ -352,17 +390,22 @@ def grouped_gemm(A: torch.Tensor, B: torch.Tensor, As: torch.Tensor, Bs: torch.T
     """Block-scaled FP8 product of each row with its expert's weights: C[r] = gemm(A[r], B[e]) for the rows r of
     expert e in `route`, bf16 or fp32 [T * k, N]. A holds the rows themselves (e.g. grouped_gemm_silu_quant's Q), or
     with gather=True the tokens. Rows past route.offsets[-1] are not written."""
-    dev, A, As, Bs, rows_a, R, hint, E, N, K = _check_grouped(A, B, As, Bs, route, b_tiled)
-    _need(gather or rows_a >= R, f"A has {rows_a} rows, the route has {R}")
+    index, A, As, Bs, rows_a, R, hint, E, N, K = _check_grouped(A, B, As, Bs, route, b_tiled)
+    if not gather and rows_a < R:
+        raise ValueError(f"A has {rows_a} rows, the route has {R}")
     if out is None:
-        out = torch.empty((R, N), dtype=out_dtype, device=dev)
-    _need(out.dtype in (torch.bfloat16, torch.float32), "output must be bf16 or fp32")
-    _need(out.device == dev and out.shape == (R, N) and out.stride(1) == 1, "output must be [T * k, N] with contiguous rows")
-    with _native.device_guard(dev):
-        _native.check(_native.lib().bs_fp8_grouped_gemm(
-            A.data_ptr(), B.data_ptr(), out.data_ptr(), As.data_ptr(), Bs.data_ptr(), route.offsets.data_ptr(),
-            route.row_token.data_ptr() if gather else None, rows_a, R, hint, E, N, K, out.stride(0) if R > 1 else N,
-            int(b_tiled), int(out.dtype == torch.float32), _native.stream_handle(dev)), "bs_fp8_grouped_gemm")
+        out = torch.empty((R, N), dtype=out_dtype, device=A.device)
+        ldc = N
+    else:
+        if out.shape != (R, N) or out.get_device() != index or out.stride(1) != 1:
+            raise ValueError("output must be [T * k, N] with contiguous rows, on the same device")
+        ldc = out.stride(0) if R > 1 else N
+    f32 = out.dtype == torch.float32
+    if not f32 and out.dtype != torch.bfloat16:
+        raise ValueError("output must be bf16 or fp32")
+    _native.call(_native.lib().bs_fp8_grouped_gemm, "bs_fp8_grouped_gemm", index, A.data_ptr(), B.data_ptr(), out.data_ptr(),
+                 As.data_ptr(), Bs.data_ptr(), route.offsets.data_ptr(), route.row_token.data_ptr() if gather else None,
+                 rows_a, R, hint, E, N, K, ldc, b_tiled, f32)
     return out
 
 
@@ -371,29 +414,35 @@ def grouped_gemm_silu_quant(A: torch.Tensor, B: torch.Tensor, As: torch.Tensor, 
     """gemm_silu_quant of each row's token with its expert's [gate; up] weights: A e4m3 [T, K] holds the tokens, read
     in place through route.row_token. Returns Q e4m3 [T * k, I] and Qs fp32 [T * k, I/128] in row order; rows
     past route.offsets[-1] are not written."""
-    dev, A, As, Bs, rows_a, R, hint, E, N2, K = _check_grouped(A, B, As, Bs, route, b_tiled)
-    _need(N2 % (2 * BLOCK) == 0, "gate_up rows must be a multiple of 256")
-    inter = N2 // 2
-    Q = torch.empty((R, inter), dtype=E4M3, device=dev)
-    Qs = torch.empty((R, inter // BLOCK), dtype=torch.float32, device=dev)
-    with _native.device_guard(dev):
-        _native.check(_native.lib().bs_fp8_grouped_gemm_silu_quant(
-            A.data_ptr(), B.data_ptr(), Q.data_ptr(), As.data_ptr(), Bs.data_ptr(), Qs.data_ptr(),
-            route.offsets.data_ptr(), route.row_token.data_ptr(), rows_a, R, hint, E, N2, K, int(b_tiled),
-            _native.stream_handle(dev)), "bs_fp8_grouped_gemm_silu_quant")
+    index, A, As, Bs, rows_a, R, hint, E, N2, K = _check_grouped(A, B, As, Bs, route, b_tiled)
+    if N2 % (2 * BLOCK):
+        raise ValueError("gate_up rows must be a multiple of 256")
+    dev = A.device
+    Q = torch.empty((R, N2 // 2), dtype=E4M3, device=dev)
+    Qs = torch.empty((R, N2 // (2 * BLOCK)), dtype=torch.float32, device=dev)
+    _native.call(_native.lib().bs_fp8_grouped_gemm_silu_quant, "bs_fp8_grouped_gemm_silu_quant", index, A.data_ptr(),
+                 B.data_ptr(), Q.data_ptr(), As.data_ptr(), Bs.data_ptr(), Qs.data_ptr(), route.offsets.data_ptr(),
+                 route.row_token.data_ptr(), rows_a, R, hint, E, N2, K, b_tiled)
     return Q, Qs
 
 
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t with contiguous rows that start on 16 bytes (a copy where they do not)."""
-    per16 = 16 // t.element_size()
-    if t.stride(-1) != 1 or (t.shape[0] > 1 and (t.stride(0) % per16 or t.stride(0) < t.shape[1])) or t.data_ptr() % 16:
-        return t.contiguous()
-    return t
+def _rows16(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """(t with contiguous rows that start on 16 bytes, copied where they do not; its row stride)."""
+    rows, n = t.shape
+    ld, inner = t.stride()
+    if rows <= 1:
+        ld = n
+    if inner != 1 or ld < n or (ld * t.element_size()) % 16 or t.data_ptr() % 16:
+        return t.clone(memory_format=torch.contiguous_format), n
+    return t, ld
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _norm_weight(w: torch.Tensor | None, H: int, index: int) -> int | None:
+    if w is None:
+        return None
+    if w.dtype != torch.bfloat16 or w.shape != (H,) or w.get_device() != index or w.stride(0) != 1 or w.data_ptr() % 16:
+        raise ValueError("norm weights must be contiguous, 16-byte aligned bf16 [H] on the same device")
+    return w.data_ptr()
 
 
 def block_norm_quant(y: torch.Tensor, residual: torch.Tensor, *, post_weight: torch.Tensor | None = None,
@@ -409,24 +458,39 @@ def block_norm_quant(y: torch.Tensor, residual: torch.Tensor, *, post_weight: to
     rounded once, into `out` (a new tensor like residual; pass out=residual to update it in place); A is
     taken from the unrounded h. Returns (h, A e4m3 [T, H], As fp32 [T, H/128]), or h alone without pre_weight."""
     bf16 = torch.bfloat16
-    _need(y.dim() == 2 and y.dtype == bf16, "y must be bf16 [rows, H]")
-    _need(residual.dim() == 2 and residual.dtype in (bf16, torch.float32), "residual must be bf16 or fp32 [T, H]")
-    dev = _cuda(y, residual)
+    wide = residual.dtype == torch.float32
+    if y.dim() != 2 or y.dtype != bf16:
+        raise ValueError("y must be bf16 [rows, H]")
+    if residual.dim() != 2 or not (wide or residual.dtype == bf16):
+        raise ValueError("residual must be bf16 or fp32 [T, H]")
+    index, dev = _one_device(y, residual), y.device
     T, H = residual.shape
-    _need(H % BLOCK == 0 and 0 < H <= 16384, "H must be a multiple of 128, at most 16384")
-    _need(y.shape[1] == H and (route is not None or y.shape[0] == T), "y must have residual's shape (or be a route's rows)")
-    y, residual = _rows16(y), _rows16(residual)
-    for w in (post_weight, pre_weight):
-        _need(w is None or (w.shape == (H,) and w.dtype == bf16 and w.device == dev and w.is_contiguous()
-                            and w.data_ptr() % 16 == 0), "norm weights must be contiguous bf16 [H] on the same device")
-    kind, ldg = 0, 0
+    rows_y, hy = y.shape
+    if H % BLOCK or not 0 < H <= 16384:
+        raise ValueError("H must be a multiple of 128, at most 16384")
+    if hy != H or (route is None and rows_y != T):
+        raise ValueError("y must have residual's shape (or be a route's rows)")
+    given = out
+    if out is None:
+        out, ldo = torch.empty((T, H), dtype=residual.dtype, device=dev), H
+    else:
+        if out.shape != (T, H) or out.dtype != residual.dtype or out.get_device() != index:
+            raise ValueError("out must be like residual")
+        same, ldo = _rows16(out)
+        if same is not out:
+            raise ValueError("out must have contiguous 16-byte aligned rows")
+    y, ldy = _rows16(y)
+    residual, ldr = (out, ldo) if residual is given else _rows16(residual)
+    post, pre = _norm_weight(post_weight, H, index), _norm_weight(pre_weight, H, index)
+    kind, ldg, g_ptr = 0, 0, None
     if gate is not None:
-        _need(gate.dtype == bf16 and gate.device == dev, "gate must be bf16 on the same device")
+        if gate.dtype != bf16 or gate.get_device() != index:
+            raise ValueError("gate must be bf16 on the same device")
         if gate.dim() == 1:
-            _need(gate.shape == (H,), "gate must be [H], [T, 1] or [T, H]")
-            kind, gate = 1, gate.contiguous()
-            if gate.data_ptr() % 16:
-                gate = gate.clone()
+            _need(gate.shape[0] == H, "gate must be [H], [T, 1] or [T, H]")
+            if gate.stride(0) != 1 or gate.data_ptr() % 16:
+                gate = gate.clone(memory_format=torch.contiguous_format)
+            kind = 1
         else:
             _need(gate.dim() == 2 and gate.shape[0] == T and gate.shape[1] in (1, H), "gate must be [H], [T, 1] or [T, H]")
             if gate.shape[1] == 1:
@@ -434,30 +498,24 @@ def block_norm_quant(y: torch.Tensor, residual: torch.Tensor, *, post_weight: to
                     gate = gate.contiguous()
                 kind, ldg = 2, gate.stride(0) if T > 1 else 1
             else:
-                gate = _rows16(gate)
-                kind, ldg = 3, _row_stride(gate)
+                kind, (gate, ldg) = 3, _rows16(gate)
+        g_ptr = gate.data_ptr()
     w_ptr = s_ptr = None
     k = 0
     if route is not None:
-        _need(route.weights is not None and route.weights.shape == route.slot_row.shape, "the route has no weights")
-        _cuda(y, route.weights, route.slot_row)
-        _need(route.weights.dtype == torch.float32 and route.weights.is_contiguous()
-              and route.slot_row.dtype == torch.int32 and route.slot_row.is_contiguous(),
-              "the route's weights and rows must be contiguous fp32 and int32")
-        _need(route.slot_row.shape[0] == T, f"the route has {route.slot_row.shape[0]} tokens, the residual {T}")
-        w_ptr, s_ptr, k = route.weights.data_ptr(), route.slot_row.data_ptr(), route.slot_row.shape[1]
-    if out is None:
-        out = torch.empty((T, H), dtype=residual.dtype, device=dev)
-    _need(out.shape == (T, H) and out.dtype == residual.dtype and out.device == dev and _rows16(out) is out,
-          "out must be like residual, with contiguous 16-byte aligned rows")
-    A = As = None
-    if pre_weight is not None:
+        w, rows = route.weights, route.slot_row
+        if w is None or w.shape != rows.shape or rows.shape[0] != T:
+            raise ValueError("the route must have weights, and a token for each row of the residual")
+        _one_device(y, w, rows)
+        if w.dtype != torch.float32 or rows.dtype != torch.int32 or not (w.is_contiguous() and rows.is_contiguous()):
+            raise ValueError("the route's weights and rows must be contiguous fp32 and int32")
+        w_ptr, s_ptr, k = w.data_ptr(), rows.data_ptr(), rows.shape[1]
+    A = As = a_ptr = as_ptr = None
+    if pre is not None:
         A = torch.empty((T, H), dtype=E4M3, device=dev)
         As = torch.empty((T, H // BLOCK), dtype=torch.float32, device=dev)
-    with _native.device_guard(dev):
-        _native.check(_native.lib().bs_fp8_block_norm_quant(
-            y.data_ptr(), _row_stride(y), y.shape[0], w_ptr, s_ptr, k, residual.data_ptr(), _row_stride(residual),
-            out.data_ptr(), _row_stride(out), int(residual.dtype == torch.float32), _native.ptr(post_weight),
-            _native.ptr(gate), kind, ldg, float(scale), float(residual_scale), _native.ptr(pre_weight), float(eps),
-            _native.ptr(A), _native.ptr(As), T, H, _native.stream_handle(dev)), "bs_fp8_block_norm_quant")
-    return out if pre_weight is None else (out, A, As)
+        a_ptr, as_ptr = A.data_ptr(), As.data_ptr()
+    _native.call(_native.lib().bs_fp8_block_norm_quant, "bs_fp8_block_norm_quant", index, y.data_ptr(), ldy, rows_y, w_ptr,
+                 s_ptr, k, residual.data_ptr(), ldr, out.data_ptr(), ldo, wide, post, g_ptr, kind, ldg, scale,
+                 residual_scale, pre, eps, a_ptr, as_ptr, T, H)
+    return out if pre is None else (out, A, As)
