@@ -523,20 +523,25 @@ __global__ void __launch_bounds__(GroupedRowsCfg<FUSED>::kThreads, 1)
 //
 // CTA layout (384 threads): warps 0-7 promotion (warpgroup g: tokens [g * NT/2, ...)) and epilogue, warp 8 TMA
 // producer, warp 9 TMEM + MMA issuer, warps 10-11 scale products As[src, kb] * Bs[nb, kb] into a ring of eight slots.
+// A unit of the pipeline is kKu K blocks of a tile (32 KB of weights): gate and up of one K block, or two K blocks of
+// one weight block, each set of partials in TMEM columns of its own.
 template <bool FUSED, int NT>
 struct GroupedTokensCfg {
   static constexpr int kThreads = 384;
   static constexpr int kNwg = FUSED ? 2 : 1;
+  static constexpr int kKu = FUSED ? 1 : 2;
+  static constexpr int kSets = kNwg * kKu;
   static constexpr int kTr = NT / 2;
-  static constexpr int kWBytes = 16384 * kNwg;
+  static constexpr int kWBytes = 16384 * kNwg;  // per K block
   static constexpr int kXBytes = NT * 128;
-  static constexpr int kStageBytes = kWBytes + ((kXBytes + 1023) / 1024) * 1024;
-  static constexpr int kBufCols = kNwg * NT;
+  static constexpr int kBlockBytes = kWBytes + ((kXBytes + 1023) / 1024) * 1024;
+  static constexpr int kStageBytes = kKu * kBlockBytes;
+  static constexpr int kBufCols = kSets * NT;
   static constexpr int kBufs = 512 / kBufCols > 4 ? 4 : 512 / kBufCols;
-  static constexpr int kTmemCols = kBufs * kBufCols < 32 ? 32 : kBufs * kBufCols;
-  static_assert((kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols <= 512, "TMEM columns");
+  static constexpr int kTmemCols = kBufs * kBufCols;
+  static_assert((kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols >= 32 && kTmemCols <= 512, "TMEM columns");
   static constexpr int kSlots = 8;
-  static constexpr int kRingBytes = kSlots * kNwg * NT * 4;
+  static constexpr int kRingBytes = kSlots * kSets * NT * 4;
   static constexpr int kXchBytes = kNwg * NT * 128 * 4;     // [S][kNwg][NT / S][128] partials
   static constexpr int kAmaxBytes = FUSED ? NT * 4 * 4 : 0;  // [own token][4 warps]
   static constexpr int kBarBytes = 512;
@@ -596,12 +601,13 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
     k_grouped_tokens(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                      const GroupedParams p, const int log_s) {
   using Cfg = GroupedTokensCfg<FUSED, NT>;
-  constexpr int ST = Cfg::kStages, NWG = Cfg::kNwg, NB = Cfg::kBufs, NS = Cfg::kSlots, TR = Cfg::kTr;
+  constexpr int ST = Cfg::kStages, NWG = Cfg::kNwg, KU = Cfg::kKu, NSET = Cfg::kSets, NB = Cfg::kBufs, NS = Cfg::kSlots,
+                TR = Cfg::kTr;
   extern __shared__ uint8_t smem_raw[];
   // (the offset of the aligned base is the same in every CTA: mapped addresses of the cluster's CTAs agree)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* xch = reinterpret_cast<float*>(smem + Cfg::kXchOff);
-  float* ring = reinterpret_cast<float*>(smem + Cfg::kRingOff);  // [NS][NWG][NT] scale products
+  float* ring = reinterpret_cast<float*>(smem + Cfg::kRingOff);  // [NS][KU][NWG][NT] scale products
   float* amx = reinterpret_cast<float*>(smem + Cfg::kAmaxOff);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::kBarOff);
   uint64_t* empty = full + ST;
@@ -678,20 +684,31 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
                          source_row(p, min(r + 3, last)));
       }
       const int nb = t.expert * nblk + t.tn;
-      for (int kb = kb0; kb < kb1; ++kb) {
+      for (int kb = kb0; kb < kb1; kb += KU) {
         if (lane == 0) ok = mbar_wait(&empty[s], ph ^ 1, abort_flag, p.status, kErrTimeoutEmpty);
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
         uint8_t* st = smem + s * Cfg::kStageBytes;
+        const int nk = min(KU, kb1 - kb);
         if (lane == 0) {
-          mbar_arrive_expect_tx(&full[s], Cfg::kWBytes + (gather ? quads * 512 : Cfg::kXBytes));
+          mbar_arrive_expect_tx(&full[s], nk * (Cfg::kWBytes + (gather ? quads * 512 : Cfg::kXBytes)));
 #pragma unroll
-          for (int w = 0; w < NWG; ++w)
-            load_weight_box(st + w * 16384, &tmW, &full[s], w == 0 ? nb : nb + I_blk, kb, KB, p.b_tiled, pol_w);
-          if (!gather) tma_load_2d(st + Cfg::kWBytes, &tmX, &full[s], kb * 128, t.row, pol_x);
+          for (int h = 0; h < KU; ++h) {
+            if (h >= nk) break;
+            uint8_t* sh = st + h * Cfg::kBlockBytes;
+#pragma unroll
+            for (int w = 0; w < NWG; ++w)
+              load_weight_box(sh + w * 16384, &tmW, &full[s], w == 0 ? nb : nb + I_blk, kb + h, KB, p.b_tiled, pol_w);
+            if (!gather) tma_load_2d(sh + Cfg::kWBytes, &tmX, &full[s], (kb + h) * 128, t.row, pol_x);
+          }
         }
         __syncwarp();
-        if (gather && lane < quads) tma_gather4(st + Cfg::kWBytes + 512 * lane, &tmX, &full[s], kb * 128, rows, pol_x);
+        if (gather && lane < quads) {
+#pragma unroll
+          for (int h = 0; h < KU; ++h)
+            if (h < nk)
+              tma_gather4(st + h * Cfg::kBlockBytes + Cfg::kWBytes + 512 * lane, &tmX, &full[s], (kb + h) * 128, rows, pol_x);
+        }
         issued |= 1u << s;
         parity_bits = (parity_bits & ~(1u << s)) | (ph << s);
         if (++s == ST) {
@@ -714,20 +731,24 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
         const GroupTile t = find_tile(table, tile, NT);
         // Columns past the tile's rows are computed from whatever the stage holds (or skipped) and never read.
         const uint32_t idesc = idesc_e4m3_f32(128, (t.rows + 15) / 16 * 16);
-        for (int kb = kb0; kb < kb1; ++kb) {
+        for (int kb = kb0; kb < kb1; kb += KU) {
           ok = mbar_wait(&full[s], ph, abort_flag, p.status, kErrTimeoutFull) &&
                mbar_wait(&pempty[b], pph ^ 1, abort_flag, p.status, kErrTimeoutPEmpty);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t st = smem_u32(smem + s * Cfg::kStageBytes);
-          const uint32_t xs = st + Cfg::kWBytes;
 #pragma unroll
-          for (int w = 0; w < NWG; ++w) {
-            const uint32_t d = tmem + static_cast<uint32_t>(b * Cfg::kBufCols + w * NT);
+          for (int h = 0; h < KU; ++h) {
+            if (kb + h >= kb1) break;
+            const uint32_t st = smem_u32(smem + s * Cfg::kStageBytes + h * Cfg::kBlockBytes);
+            const uint32_t xs = st + Cfg::kWBytes;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mma_e4m3(d, desc_kmajor_sw128(st + w * 16384 + 32 * k), desc_kmajor_sw128(xs + 32 * k), idesc,
-                       k > 0 ? 1u : 0u);
+            for (int w = 0; w < NWG; ++w) {
+              const uint32_t d = tmem + static_cast<uint32_t>(b * Cfg::kBufCols + (h * NWG + w) * NT);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mma_e4m3(d, desc_kmajor_sw128(st + w * 16384 + 32 * k), desc_kmajor_sw128(xs + 32 * k), idesc,
+                         k > 0 ? 1u : 0u);
+            }
           }
           mma_commit(&empty[s]);
           mma_commit(&pfull[b]);
@@ -761,28 +782,34 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
       }
       const float* brow = p.Bs + (static_cast<size_t>(t.expert) * nblk + t.tn) * KB;
       const float* urow = brow + static_cast<size_t>(I_blk) * KB;
-      float a[2][TPL], bw[2][NWG];  // operands of this K block and the next
-      auto load = [&](int h, int kb) {
+      float a[2][KU][TPL], bw[2][KU][NWG];  // operands of this unit and the next
+      auto load = [&](int u, int kb) {
 #pragma unroll
-        for (int j = 0; j < TPL; ++j) a[h][j] = ldg_f32(arow[j] + kb);
+        for (int h = 0; h < KU; ++h) {
+          const int k = min(kb + h, kb1 - 1);
 #pragma unroll
-        for (int w = 0; w < NWG; ++w) bw[h][w] = ldg_f32((w == 0 ? brow : urow) + kb);
+          for (int j = 0; j < TPL; ++j) a[u][h][j] = ldg_f32(arow[j] + k);
+#pragma unroll
+          for (int w = 0; w < NWG; ++w) bw[u][h][w] = ldg_f32((w == 0 ? brow : urow) + k);
+        }
       };
-      auto write = [&](int h, int kb_next) {
+      auto write = [&](int u, int kb_next) {
         if (!mbar_wait(&sempty[slot], sph ^ 1, abort_flag, p.status, kErrTimeoutPEmpty)) {
           ok = false;
           return;
         }
-        float* dst = ring + slot * (NWG * NT);
+        float* dst = ring + slot * (NSET * NT);
 #pragma unroll
-        for (int w = 0; w < NWG; ++w)
+        for (int h = 0; h < KU; ++h)
 #pragma unroll
-          for (int j = 0; j < TPL; ++j) {
-            const int tok = tok_base + 32 * j;
-            if (tok < NT) dst[w * NT + tok] = tok < t.rows ? __fmul_rn(a[h][j], bw[h][w]) : 0.f;
-          }
+          for (int w = 0; w < NWG; ++w)
+#pragma unroll
+            for (int j = 0; j < TPL; ++j) {
+              const int tok = tok_base + 32 * j;
+              if (tok < NT) dst[(h * NWG + w) * NT + tok] = tok < t.rows ? __fmul_rn(a[u][h][j], bw[u][h][w]) : 0.f;
+            }
         mbar_arrive(&sfull[slot]);
-        load(h, kb_next);
+        load(u, kb_next);
         if (++slot == NS) {
           slot = 0;
           sph ^= 1;
@@ -790,11 +817,11 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
       };
       if (kb0 < kb1) {
         load(0, kb0);
-        load(1, min(kb0 + 1, kb1 - 1));
+        load(1, min(kb0 + KU, kb1 - 1));
       }
-      for (int kb = kb0; kb < kb1 && ok; kb += 2) {
-        write(0, min(kb + 2, kb1 - 1));
-        if (kb + 1 < kb1 && ok) write(1, min(kb + 3, kb1 - 1));
+      for (int kb = kb0; kb < kb1 && ok; kb += 2 * KU) {
+        write(0, min(kb + 2 * KU, kb1 - 1));
+        if (kb + KU < kb1 && ok) write(1, min(kb + 3 * KU, kb1 - 1));
       }
     }
   } else {
@@ -816,34 +843,37 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
       for (int w = 0; w < NWG; ++w)
 #pragma unroll
         for (int i = 0; i < TR / 2; ++i) acc[w][i] = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
+      for (int kb = kb0; kb < kb1; kb += KU) {
         if (ok && !(mbar_wait_warp(&pfull[b], pph, abort_flag, p.status, kErrTimeoutPFull) &&
                     mbar_wait_warp(&sfull[slot], sph, abort_flag, p.status, kErrTimeoutPFull)))
           ok = false;
         if (ok) {
           tc_fence_after();
           const uint32_t tb = tmem + lane_addr + static_cast<uint32_t>(b * Cfg::kBufCols + tok0);
-          const ulonglong2* sc = reinterpret_cast<const ulonglong2*>(ring + slot * (NWG * NT) + tok0);
+          const ulonglong2* sc = reinterpret_cast<const ulonglong2*>(ring + slot * (NSET * NT) + tok0);
           constexpr int CH = TR < 16 ? TR : 16;  // columns skipped together when the tile has no such tokens
-          uint32_t v[NWG][TR];
+          uint32_t v[NSET][TR];
 #pragma unroll
           for (int c0 = 0; c0 < TR; c0 += CH)
             if (tok0 + c0 < n) {
 #pragma unroll
-              for (int w = 0; w < NWG; ++w) tmem_ld_run<CH>(tb + w * NT + c0, v[w] + c0);
+              for (int w = 0; w < NSET; ++w) tmem_ld_run<CH>(tb + w * NT + c0, v[w] + c0);
             }
           tmem_ld_wait();
           mbar_arrive(&pempty[b]);
+          const bool whole = kb + KU <= kb1;  // else the unit's last sets hold an earlier unit's values
 #pragma unroll
           for (int c0 = 0; c0 < TR; c0 += CH)
             if (tok0 + c0 < n) {
 #pragma unroll
-              for (int w = 0; w < NWG; ++w)
+              for (int w = 0; w < NSET; ++w)
+                if (w < NWG || whole) {
 #pragma unroll
-                for (int i = c0; i < c0 + CH; i += 4) {
-                  const ulonglong2 s2 = sc[(w * NT + i) / 4];
-                  ffma2(acc[w][i / 2], v[w][i], v[w][i + 1], s2.x);
-                  ffma2(acc[w][i / 2 + 1], v[w][i + 2], v[w][i + 3], s2.y);
+                  for (int i = c0; i < c0 + CH; i += 4) {
+                    const ulonglong2 s2 = sc[(w * NT + i) / 4];
+                    ffma2(acc[w % NWG][i / 2], v[w][i], v[w][i + 1], s2.x);
+                    ffma2(acc[w % NWG][i / 2 + 1], v[w][i + 2], v[w][i + 3], s2.y);
+                  }
                 }
             }
           mbar_arrive(&sempty[slot]);
@@ -858,23 +888,37 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
         }
       }
 
-      // ---------------- partials to the tokens' owners
-      if (ok && !mbar_wait_cluster(rempty, rph ^ 1, abort_flag, p.status)) ok = false;
-      if (ok) {
+      // ---------------- partials to the tokens' owners. Alone, a CTA needs no more than its own barrier for it.
+      if (log_s == 0) {
+        named_bar_sync(3, 256);  // every warp has read the previous tile's
+        if (ok) {
 #pragma unroll
-        for (int i = 0; i < TR; ++i) {
-          const int tok = tok0 + i;
-          if (tok < n) {
-            const int to = tok & (S - 1);
+          for (int i = 0; i < TR; ++i)
+            if (tok0 + i < n) {
 #pragma unroll
-            for (int w = 0; w < NWG; ++w)
-              st_cluster_f32(mapa_shared(xch + ((rank * NWG + w) * own + (tok >> log_s)) * 128 + r, to),
-                             (i & 1) ? hi_f(acc[w][i / 2]) : lo_f(acc[w][i / 2]));
-          }
+              for (int w = 0; w < NWG; ++w)
+                xch[(w * NT + tok0 + i) * 128 + r] = (i & 1) ? hi_f(acc[w][i / 2]) : lo_f(acc[w][i / 2]);
+            }
         }
-        __syncwarp();
-        if (lane < S) mbar_arrive_cluster(mapa_shared(rfull, lane));
-        if (!mbar_wait_cluster(rfull, rph, abort_flag, p.status)) ok = false;
+        named_bar_sync(3, 256);
+      } else if (ok) {
+        ok = mbar_wait_cluster(rempty, rph ^ 1, abort_flag, p.status);
+        if (ok) {
+#pragma unroll
+          for (int i = 0; i < TR; ++i) {
+            const int tok = tok0 + i;
+            if (tok < n) {
+              const int to = tok & (S - 1);
+#pragma unroll
+              for (int w = 0; w < NWG; ++w)
+                st_cluster_f32(mapa_shared(xch + ((rank * NWG + w) * own + (tok >> log_s)) * 128 + r, to),
+                               (i & 1) ? hi_f(acc[w][i / 2]) : lo_f(acc[w][i / 2]));
+            }
+          }
+          __syncwarp();
+          if (lane < S) mbar_arrive_cluster(mapa_shared(rfull, lane));
+          ok = mbar_wait_cluster(rfull, rph, abort_flag, p.status);
+        }
       }
       // ---------------- this CTA's tokens: rank, rank + S, ... below n
       const int n_own = n > rank ? (n - rank + S - 1) >> log_s : 0;
@@ -926,7 +970,7 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
           }
         }
       }
-      if (ok) {
+      if (ok && log_s > 0) {
         __syncwarp();
         if (lane < S) mbar_arrive_cluster(mapa_shared(rempty, lane));
       }
