@@ -559,12 +559,11 @@ struct GroupedTokensCfg {
   static constexpr int kSmemBytes = (kUsed > 120 * 1024 ? kUsed : 120 * 1024) + 1024;
 };
 
-__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
-}
-// Arrival on a barrier of any CTA of the cluster; publishes this thread's earlier writes (and what it has seen) there.
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+// A word into a CTA of the cluster; its 4 bytes are counted on that CTA's barrier `bar` when they have arrived.
+__device__ __forceinline__ void st_async_f32(uint32_t addr, float v, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr),
+               "r"(__float_as_uint(v)), "r"(bar)
+               : "memory");
 }
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -641,7 +640,7 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
       mbar_init(&sempty[i], 256);
     }
     mbar_init(drain, 1);
-    mbar_init(rfull, 8 * S);
+    mbar_init(rfull, 1);
     mbar_init(rempty, 8 * S);
     *abort_flag = 0;
     fence_mbar_init();
@@ -888,6 +887,7 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
         }
       }
 
+      const int n_own = n > rank ? (n - rank + S - 1) >> log_s : 0;  // tokens this CTA finishes: rank, rank + S, ...
       // ---------------- partials to the tokens' owners. Alone, a CTA needs no more than its own barrier for it.
       if (log_s == 0) {
         named_bar_sync(3, 256);  // every warp has read the previous tile's
@@ -902,26 +902,26 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
         }
         named_bar_sync(3, 256);
       } else if (ok) {
-        ok = mbar_wait_cluster(rempty, rph ^ 1, abort_flag, p.status);
+        // The owner's barrier counts the bytes, so no fence stands between the words and their reader.
+        if (threadIdx.x == 0) mbar_arrive_expect_tx(rfull, n_own * S * NWG * 512);
+        ok = mbar_wait_warp(rempty, rph ^ 1, abort_flag, p.status, kErrTimeoutCluster);
         if (ok) {
 #pragma unroll
           for (int i = 0; i < TR; ++i) {
             const int tok = tok0 + i;
             if (tok < n) {
               const int to = tok & (S - 1);
+              const uint32_t bar = mapa_shared(rfull, to);
 #pragma unroll
               for (int w = 0; w < NWG; ++w)
-                st_cluster_f32(mapa_shared(xch + ((rank * NWG + w) * own + (tok >> log_s)) * 128 + r, to),
-                               (i & 1) ? hi_f(acc[w][i / 2]) : lo_f(acc[w][i / 2]));
+                st_async_f32(mapa_shared(xch + ((rank * NWG + w) * own + (tok >> log_s)) * 128 + r, to),
+                             (i & 1) ? hi_f(acc[w][i / 2]) : lo_f(acc[w][i / 2]), bar);
             }
           }
-          __syncwarp();
-          if (lane < S) mbar_arrive_cluster(mapa_shared(rfull, lane));
           ok = mbar_wait_cluster(rfull, rph, abort_flag, p.status);
         }
       }
-      // ---------------- this CTA's tokens: rank, rank + S, ... below n
-      const int n_own = n > rank ? (n - rank + S - 1) >> log_s : 0;
+      // ---------------- this CTA's tokens
       if constexpr (!FUSED) {
         if (ok) {
           for (int j = warp; j < n_own; j += 8) {
@@ -971,8 +971,9 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
         }
       }
       if (ok && log_s > 0) {
+        // This warp's reads are done (their values are in the stores above): the count alone is enough.
         __syncwarp();
-        if (lane < S) mbar_arrive_cluster(mapa_shared(rempty, lane));
+        if (lane < S) mbar_arrive_remote_relaxed(mapa_shared(rempty, lane));
       }
       rph ^= 1;
     }
