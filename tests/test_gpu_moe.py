@@ -138,7 +138,7 @@ COUNTS = {"one": [0, 1, 0], "few": [3, 0, 1, 16, 17, 0, 2], "edges": [15, 16, 17
 
 
 @pytest.mark.parametrize("counts", sorted(COUNTS))
-@pytest.mark.parametrize("mean", [1, 20, 50, 0])
+@pytest.mark.parametrize("mean", [1, 10, 20, 50, 0])
 @pytest.mark.parametrize("N,K,tiled", [(128, 128, False), (384, 640, True), (640, 1152, False)])
 def test_grouped_gemm(cuda_lib, counts, mean, N, K, tiled):
     """Every kernel variant (mean rows per expert) at row counts around its tiles, rows of no expert in between, an
@@ -166,7 +166,7 @@ def test_grouped_gemm(cuda_lib, counts, mean, N, K, tiled):
 
 
 @pytest.mark.parametrize("counts", sorted(COUNTS))
-@pytest.mark.parametrize("mean", [1, 20, 50, 0])
+@pytest.mark.parametrize("mean", [1, 10, 20, 50, 0])
 @pytest.mark.parametrize("inter,K,tiled", [(128, 128, True), (384, 640, False)])
 def test_grouped_gemm_silu_quant(cuda_lib, counts, mean, inter, K, tiled):
     ops = _ops()

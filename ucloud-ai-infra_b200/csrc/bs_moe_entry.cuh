@@ -51,14 +51,28 @@ struct GroupedPlan {
   int log_s;  // k_grouped_tokens: log2 of the CTAs per tile
 };
 
+// Chosen by the mean rows per expert. Measured with router-like skew (times in us; 64 experts, 5120 -> 2 x 1024 fused,
+// 1024 -> 5120 plain; 128 experts, 2048 -> 2 x 768, 768 -> 2048; token tiles of 16 and 32 rows, row tiles):
+//   fused  mean 4.0: 97.8, 98.3, 129 (64 experts)    4.7: 58.7, 57.3, 75.8 (128)    7.6: 106, 101, 135 (64)
+//          mean 18.8: 103, 86.4, 84.8 (128)   20: 153, 127, 137 (64)   30: 209, 160, 138 (64)
+//   plain  mean 4.0: 53.0, 54.4, 57.4 (64)    4.7: 38.3, 35.6, 38.0 (128)   11.2: 50.0, 43.7, 44.2 (128)
+//          mean 12.5: 74.3, 64.0, 65.6 (64)   18.8: 65.7, 49.9, 44.9 (128)  20: 96.5, 72.4, 66.7 (64)
+// (token tiles of 64 rows were never more than 1 us ahead of the better of 32 and row tiles: not built).
+// CTAs per tile: a call with fewer tiles than SMs takes as many as fill them, with at least 8 K blocks each (36 tiles of
+// 16 K blocks: 14.6 us on one CTA each, 11.2 on two, 12.0 on four; 64 tiles of 40: 27.7, 19.3, 19.4). With more
+// tiles than SMs the fused product is faster on two (its last wave is half as long: 61 tokens 114 -> 101 us, 32
+// tokens 109 -> 98 us), the plain one on one (its tiles are too short for the exchange: 240 tokens 43.3 -> 65 us).
 GroupedPlan grouped_plan(bool fused, int E, int nblk, int KB, int rows, int num_sms) {
   GroupedPlan g = {0, 0};
-  const int mean = (rows + E - 1) / E;
-  g.nt = mean <= 12 ? 16 : mean <= 28 ? 32 : mean <= 64 ? 64 : 0;
+  const long long r = rows;
+  if (r <= 4ll * E) g.nt = 16;
+  else if (r <= (fused ? 18ll : 14ll) * E) g.nt = 32;
   if (!g.nt) return g;
-  const int active = rows < E ? rows : E;
-  const int tiles = active * (fused ? nblk / 2 : nblk);
-  while (g.log_s < 3 && (2 << g.log_s) <= KB && (tiles << g.log_s) < 4 * num_sms) ++g.log_s;
+  const long long tiles = static_cast<long long>(rows < E ? rows : E) * (fused ? nblk / 2 : nblk);
+  if (tiles > num_sms)
+    g.log_s = fused && KB >= 16 ? 1 : 0;
+  else
+    while (g.log_s < 3 && (16 << g.log_s) <= KB && (tiles << (g.log_s + 1)) <= num_sms) ++g.log_s;
   return g;
 }
 
@@ -86,7 +100,6 @@ int run_grouped(const void* A, const void* B, const bs::GroupedParams& p, int ro
   switch (g.nt) {
     case 16: return launch_grouped_tokens<FUSED, 16>(tmB, tmA, p, g.log_s, num_sms, s);
     case 32: return launch_grouped_tokens<FUSED, 32>(tmB, tmA, p, g.log_s, num_sms, s);
-    case 64: return launch_grouped_tokens<FUSED, 64>(tmB, tmA, p, g.log_s, num_sms, s);
     default: break;
   }
   using Cfg = bs::GroupedRowsCfg<FUSED>;
