@@ -8,17 +8,22 @@
 // Every step is fp32; h is rounded once to the residual's type when it is stored, and v is taken from the unrounded
 // h and goes to e4m3 without a rounding to bf16 between.
 //
-// Bound: HBM. Per token k (or 1) rows of bf16 and the residual are read, the residual and the e4m3 row written. A CTA
-// owns a row, a thread C 16-byte chunks of it (chunk c = t + blockDim * j), so z and h stay in registers between the
-// two norms, and a 128-group is the 16 chunks of a half-warp.
+// Bound: HBM. Per token k (or 1) rows of bf16 and the residual are read, the residual and the e4m3 row written; what
+// costs is keeping enough of those reads in flight beside two reductions per row, in few instructions per element. A
+// producer warp brings the rows of the CTA's next tokens into a ring in shared memory by bulk copies, up to four rows
+// per stage, whatever the other warps are doing; two CTAs per SM, about 100 KB of ring each. The other warps own C
+// 16-byte chunks of a row each (chunk c = t + threads * j), add the ring's rows up as they land, and keep z and h in
+// registers between the two norms; a 128-group is the 16 chunks of a half-warp. Measured on the way (T = 8192,
+// H = 5120, k = 8): loads into registers by four CTAs of 320 threads 218 us; the ring with a stage per row 201 us, bound
+// by the issue of 1600 instructions per warp and token (waits, IEEE divisions and square roots among them).
 #pragma once
 #include "bs_common.cuh"
 #include "bs_quant.cuh"
 
 namespace bs {
 
-constexpr int kBlockMaxThreads = 512;
-constexpr int kBlockMaxChunks = 4;  // rows of at most 512 * 4 * 8 = 16384 elements
+constexpr int kBlockMaxThreads = 320;  // that own chunks, beside the producer warp
+constexpr int kBlockMaxH = 16384;
 
 enum : int { kGateNone = 0, kGateChannel = 1, kGateToken = 2, kGateFull = 3 };
 
@@ -39,153 +44,309 @@ struct BlockParams {
   long long ldg;             // row stride of a token or full gate
   float scale, residual_scale;
   const __nv_bfloat16* pre;  // [H] or nullptr: no A, As
-  float eps;
+  float eps, inv_h;          // inv_h: 1 / H
   uint8_t* A;                // [T, H]
   float* As;                 // [T, H / 128]
   int T, H;
+  int* status;
 };
 
-// Sum over the CTA in a fixed order: a butterfly per warp, then the warp totals in warp order. `buf` is not reused
-// before the next barrier of the caller.
-__device__ __forceinline__ float block_sum(float v, float* buf) {
+constexpr int kBlockMaxStages = 16;
+constexpr int kBlockRingBytes = 100 * 1024;  // two CTAs per SM
+
+// Rows per stage (a power of two, at least two stages fit) and stages.
+__host__ __device__ inline int block_stage_rows(int k, int H) {
+  int g = k >= 3 ? 4 : k;
+  while (g > 1 && 2 * g * 2 * H > kBlockRingBytes) g >>= 1;
+  return g;
+}
+__host__ __device__ inline int block_stages(int rows, int H) {
+  const int n = kBlockRingBytes / (rows * 2 * H);
+  return n > kBlockMaxStages ? kBlockMaxStages : n;
+}
+
+// Sum over the `threads` consumer threads in a fixed order: a butterfly per warp, then one over the (at most 16) warp totals.
+// `buf` is not reused before the next barrier.
+__device__ __forceinline__ float block_sum(float v, float* buf, int threads) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float s = buf[0];
-  for (int i = 1; i < static_cast<int>(blockDim.x >> 5); ++i) s += buf[i];
-  return s;
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) buf[threadIdx.x >> 5] = v;
+  named_bar_sync(1, threads);
+  float s = lane < (threads >> 5) ? buf[lane] : 0.f;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return __shfl_sync(0xffffffffu, s, 0);
+}
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
+      : "memory");
+}
+
+// blockDim = threads that own chunks + the producer warp.
+// amax / 448, correctly rounded by one correction step (bs_quant.cuh, group_scale), without its floor.
+__device__ __forceinline__ float amax_div_448(float amax) {
+  constexpr float kInv448 = 1.0f / 448.0f;
+  const float q0 = __fmul_rn(amax, kInv448);
+  return __fmaf_rn(__fmaf_rn(-448.0f, q0, amax), kInv448, q0);
 }
 
 template <int C, bool WIDE>
-__global__ void __launch_bounds__(kBlockMaxThreads) k_block_norm(const BlockParams p) {
+__global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block_norm(const BlockParams p) {
+  extern __shared__ __align__(128) uint8_t ring[];  // [stages][G rows][2 H]
   __shared__ float sums[2][2][kBlockMaxThreads / 32];  // by row parity and norm
-  const int t = threadIdx.x, nt = blockDim.x, lane = t & 31;
-  const int nch = p.H / 8;
-  if (t == 0) grid_dep_launch();
+  __shared__ uint64_t full[kBlockMaxStages], empty[kBlockMaxStages];
+  __shared__ float4 weight[kBlockMaxStages];
+  __shared__ int there[kBlockMaxStages];  // bit g: row g of the stage is one (its slot has a row)
+  __shared__ volatile int abort_flag;
+  const int t = threadIdx.x, nt = static_cast<int>(blockDim.x) - 32, lane = t & 31;
+  const int nch = p.H / 8, row_bytes = 2 * p.H;
+  const int k = p.weights ? p.k : 1;
+  const int G = block_stage_rows(k, p.H), stages = block_stages(G, p.H);
+  if (t == 0) {
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&full[i], 2);  // both by the producer: the bytes to come, and the weights
+      mbar_init(&empty[i], nt / 32);
+    }
+    abort_flag = 0;
+    fence_mbar_init();
+    grid_dep_launch();
+  }
+  __syncthreads();
   grid_dep_wait();
-  for (int row = blockIdx.x, parity = 0; row < p.T; row += gridDim.x, parity ^= 1) {
-    float z[C][8];
-    if (p.weights) {
-#pragma unroll
-      for (int j = 0; j < C; ++j)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[j][e] = 0.f;
-      const long long at = static_cast<long long>(row) * p.k;
-#pragma unroll 4
-      for (int s = 0; s < p.k; ++s) {
-        const int r = __ldg(p.slot_row + at + s);
-        if (static_cast<unsigned>(r) >= static_cast<unsigned>(p.rows_y)) continue;
-        const float w = __ldg(p.weights + at + s);
-        const __nv_bfloat16* src = p.y + static_cast<long long>(r) * p.ldy;
-#pragma unroll
-        for (int j = 0; j < C; ++j) {
-          const int c = t + nt * j;
-          if (c < nch) {
-            float v[8];
-            unpack_bf16x8(__ldg(reinterpret_cast<const uint4*>(src + c * 8)), v);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) z[j][e] = fmaf(w, v[e], z[j][e]);
+
+  if (t >= nt) {
+    // ------------------------------------------------------------ producer
+    const uint64_t policy = policy_evict_first();
+    int st = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    // lane s holds slot s of the next token
+    auto slot = [&](int row, int& r, float& w) {
+      r = -1;
+      w = 1.f;
+      if (row >= p.T || lane >= k) return;
+      if (p.weights) {
+        r = __ldg(p.slot_row + static_cast<long long>(row) * k + lane);
+        w = __ldg(p.weights + static_cast<long long>(row) * k + lane);
+      } else {
+        r = row;
+      }
+    };
+    int next_r;
+    float next_w;
+    slot(blockIdx.x, next_r, next_w);
+    for (int row = blockIdx.x; ok && row < p.T; row += gridDim.x) {
+      const int my_r = next_r;
+      const float my_w = next_w;
+      slot(row + gridDim.x, next_r, next_w);
+      const uint32_t has = __ballot_sync(0xffffffffu, static_cast<unsigned>(my_r) < static_cast<unsigned>(p.rows_y));
+      for (int s = 0; s < k; s += G) {
+        if (lane == 0) ok = mbar_wait(&empty[st], ph ^ 1, &abort_flag, p.status, kErrTimeoutEmpty);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        // lanes s .. s + G - 1 bring their slots' rows (lanes from k on have none)
+        const uint32_t mask = (has >> s) & ((1u << G) - 1);
+        const int g = lane - s;
+        if (lane == 0) {
+          there[st] = static_cast<int>(mask);
+          mbar_arrive_expect_tx(&full[st], __popc(mask) * row_bytes);
+        }
+        if (g >= 0 && g < G) {
+          reinterpret_cast<float*>(&weight[st])[g] = my_w;
+          if ((mask >> g) & 1) {
+            bulk_load(ring + static_cast<size_t>(st * G + g) * row_bytes, p.y + static_cast<long long>(my_r) * p.ldy,
+                      row_bytes, &full[st], policy);
           }
         }
-      }
-    } else {
-      const __nv_bfloat16* src = p.y + static_cast<long long>(row) * p.ldy;
-#pragma unroll
-      for (int j = 0; j < C; ++j) {
-        const int c = t + nt * j;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[j][e] = 0.f;
-        if (c < nch) unpack_bf16x8(__ldg(reinterpret_cast<const uint4*>(src + c * 8)), z[j]);
-      }
-    }
-    if (p.post) {
-      float ss = 0.f;
-#pragma unroll
-      for (int j = 0; j < C; ++j)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(z[j][e], z[j][e], ss);
-      ss = block_sum(ss, sums[parity][0]);
-      const float rs = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, static_cast<float>(p.H)) + p.eps));
-#pragma unroll
-      for (int j = 0; j < C; ++j) {
-        const int c = t + nt * j;
-        if (c < nch) {
-          float w[8];
-          unpack_bf16x8(__ldg(reinterpret_cast<const uint4*>(p.post + c * 8)), w);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) z[j][e] = z[j][e] * rs * w[e];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[st]);  // the weights are there too
+        if (++st == stages) {
+          st = 0;
+          ph ^= 1;
         }
       }
     }
-    const float gt = p.gate_kind == kGateToken ? __bfloat162float(__ldg(p.gate + row * p.ldg)) * p.scale : p.scale;
-    float ss = 0.f;
+    if (!ok) pause_ns(2000000ull);  // copies in flight land within microseconds
+    return;
+  }
+
+  // -------------------------------------------------------------- rows
+  // What every row uses, the norm weights' and a channel gate's chunks of this thread, stays in registers where a
+  // thread has one chunk; wider rows read it again (from L1), and two CTAs fit on an SM.
+  constexpr bool kKeep = C <= 1;
+  uint4 post[kKeep ? C : 1], pre[kKeep ? C : 1], gch[kKeep ? C : 1];
+  auto chunk = [&](const __nv_bfloat16* w, int c) {
+    return w && c < nch ? __ldg(reinterpret_cast<const uint4*>(w + c * 8)) : make_uint4(0, 0, 0, 0);
+  };
+  const __nv_bfloat16* channel = p.gate_kind == kGateChannel ? p.gate : nullptr;
+  if constexpr (kKeep) {
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      post[j] = chunk(p.post, t + nt * j);
+      pre[j] = chunk(p.pre, t + nt * j);
+      gch[j] = chunk(channel, t + nt * j);
+    }
+  }
+  int st = 0;
+  uint32_t ph = 0;
+  bool ok = true;
+  for (int row = blockIdx.x, parity = 0; row < p.T; row += gridDim.x, parity ^= 1) {
+    // in flight while the rows are added up
+    uint4 res[C][WIDE ? 2 : 1], gv[kKeep ? C : 1];
+    float gt = p.scale;
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const int c = t + nt * j;
       if (c < nch) {
-        float g[8], r[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] = gt;
-        if (p.gate_kind == kGateChannel || p.gate_kind == kGateFull) {
-          const __nv_bfloat16* gr = p.gate + (p.gate_kind == kGateFull ? row * p.ldg : 0) + c * 8;
-          unpack_bf16x8(__ldg(reinterpret_cast<const uint4*>(gr)), g);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) g[e] *= p.scale;
-        }
         if constexpr (WIDE) {
-          const float4* rr = reinterpret_cast<const float4*>(static_cast<const float*>(p.residual) + row * p.ldr + c * 8);
-          const float4 a = rr[0], b = rr[1];
-          r[0] = a.x, r[1] = a.y, r[2] = a.z, r[3] = a.w, r[4] = b.x, r[5] = b.y, r[6] = b.z, r[7] = b.w;
+          const uint4* rr = reinterpret_cast<const uint4*>(static_cast<const float*>(p.residual) + row * p.ldr + c * 8);
+          res[j][0] = rr[0];
+          res[j][1] = rr[1];
         } else {
-          unpack_bf16x8(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.residual) + row * p.ldr + c * 8), r);
+          res[j][0] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.residual) + row * p.ldr + c * 8);
         }
+        if constexpr (kKeep) gv[j] = p.gate_kind == kGateFull ? chunk(p.gate + row * p.ldg, c) : gch[j];
+      }
+    }
+    if (p.gate_kind == kGateToken) gt = __bfloat162float(__ldg(p.gate + row * p.ldg)) * p.scale;
+
+    uint64_t z[C][4];  // pairs of this thread's elements
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          z[j][e] = fmaf(g[e], z[j][e], p.residual_scale * r[e]);
-          ss = fmaf(z[j][e], z[j][e], ss);
+    for (int j = 0; j < C; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[j][e] = 0;
+    for (int s = 0; s < k; s += G) {
+      if (ok) ok = mbar_wait_warp(&full[st], ph, &abort_flag, p.status, kErrTimeoutFull);
+      if (ok) {
+        const int mask = there[st];
+        const float4 w4 = weight[st];
+        const float w[4] = {w4.x, w4.y, w4.z, w4.w};
+        const uint8_t* src = ring + static_cast<size_t>(st * G) * row_bytes + t * 16;
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+          if (t + nt * j < nch) {
+            uint4 v[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+              if ((mask >> g) & 1) v[g] = *reinterpret_cast<const uint4*>(src + g * row_bytes + nt * j * 16);
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+              if ((mask >> g) & 1) {
+                const uint64_t w2 = pack_f2(w[g], w[g]);
+                z[j][0] = ffma2r(w2, bf16x2_to_f2(v[g].x), z[j][0]);
+                z[j][1] = ffma2r(w2, bf16x2_to_f2(v[g].y), z[j][1]);
+                z[j][2] = ffma2r(w2, bf16x2_to_f2(v[g].z), z[j][2]);
+                z[j][3] = ffma2r(w2, bf16x2_to_f2(v[g].w), z[j][3]);
+              }
+          }
         }
-        if constexpr (WIDE) {
-          float4* oo = reinterpret_cast<float4*>(static_cast<float*>(p.out) + row * p.ldo + c * 8);
-          oo[0] = make_float4(z[j][0], z[j][1], z[j][2], z[j][3]);
-          oo[1] = make_float4(z[j][4], z[j][5], z[j][6], z[j][7]);
-        } else {
-          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + row * p.ldo + c * 8) =
-              make_uint4(pack_bf16x2(z[j][0], z[j][1]), pack_bf16x2(z[j][2], z[j][3]), pack_bf16x2(z[j][4], z[j][5]),
-                         pack_bf16x2(z[j][6], z[j][7]));
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+      if (++st == stages) {
+        st = 0;
+        ph ^= 1;
+      }
+    }
+    auto square_sum = [&](float* buf) {
+      uint64_t ss2 = 0;
+#pragma unroll
+      for (int j = 0; j < C; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ss2 = ffma2r(z[j][e], z[j][e], ss2);  // zero past the row's end
+      const float ss = block_sum(lo_f(ss2) + hi_f(ss2), buf, nt);
+      return rsqrtf(fmaf(ss, p.inv_h, p.eps));
+    };
+    if (p.post) {
+      const float rs = square_sum(sums[parity][0]);
+      const uint64_t rs2 = pack_f2(rs, rs);
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        const uint4 wv = kKeep ? post[kKeep ? j : 0] : chunk(p.post, t + nt * j);
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&wv);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[j][e] = fmul2(fmul2(z[j][e], rs2), bf16x2_to_f2(w[e]));
+      }
+    }
+    const uint64_t gs2 = pack_f2(gt, gt), a2 = pack_f2(p.residual_scale, p.residual_scale);
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      const int c = t + nt * j;
+      if (c < nch) {
+        uint4 g4;
+        if constexpr (kKeep) g4 = gv[j];
+        else g4 = chunk(p.gate_kind == kGateFull ? p.gate + row * p.ldg : channel, c);
+        const uint32_t* gw = reinterpret_cast<const uint32_t*>(&g4);
+        const uint32_t* rw = reinterpret_cast<const uint32_t*>(&res[j][0]);
+        const bool per_element = p.gate_kind == kGateChannel || p.gate_kind == kGateFull;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint64_t g = per_element ? fmul2(bf16x2_to_f2(gw[e]), gs2) : gs2;
+          uint64_t r;
+          if constexpr (WIDE) {
+            const uint32_t* ww = reinterpret_cast<const uint32_t*>(&res[j][e >> 1]);
+            r = static_cast<uint64_t>(ww[(2 * e) & 3]) | (static_cast<uint64_t>(ww[(2 * e + 1) & 3]) << 32);
+          } else {
+            r = bf16x2_to_f2(rw[e]);
+          }
+          z[j][e] = ffma2r(g, z[j][e], fmul2(a2, r));
+        }
+        if (ok) {
+          if constexpr (WIDE) {
+            float4* oo = reinterpret_cast<float4*>(static_cast<float*>(p.out) + row * p.ldo + c * 8);
+            oo[0] = make_float4(lo_f(z[j][0]), hi_f(z[j][0]), lo_f(z[j][1]), hi_f(z[j][1]));
+            oo[1] = make_float4(lo_f(z[j][2]), hi_f(z[j][2]), lo_f(z[j][3]), hi_f(z[j][3]));
+          } else {
+            *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + row * p.ldo + c * 8) =
+                make_uint4(pack_bf16x2(lo_f(z[j][0]), hi_f(z[j][0])), pack_bf16x2(lo_f(z[j][1]), hi_f(z[j][1])),
+                           pack_bf16x2(lo_f(z[j][2]), hi_f(z[j][2])), pack_bf16x2(lo_f(z[j][3]), hi_f(z[j][3])));
+          }
         }
       }
     }
     if (p.pre) {
-      ss = block_sum(ss, sums[parity][1]);
-      const float rs = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, static_cast<float>(p.H)) + p.eps));
+      // v = u * rs with u = h * pre. The quotient v / As is u / (amax(u) / 448), so the row's 1 / sqrt only enters As,
+      // and the bytes see one rounding (of u) before the division; rows so small that As is at its floor divide
+      // u * rs by the floor.
+      const float rs = square_sum(sums[parity][1]);
 #pragma unroll
       for (int j = 0; j < C; ++j) {
         if (nt * j >= nch) break;  // uniform across the CTA
         const int c = t + nt * j;
-        const bool active = c < nch;
+        const uint4 wv = kKeep ? pre[kKeep ? j : 0] : chunk(p.pre, c);
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&wv);
         float amax = 0.f;
-        if (active) {
-          float w[8];
-          unpack_bf16x8(__ldg(reinterpret_cast<const uint4*>(p.pre + c * 8)), w);
+        uint64_t u[4];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            z[j][e] = z[j][e] * rs * w[e];
-            amax = fmaxf(amax, fabsf(z[j][e]));
-          }
+        for (int e = 0; e < 4; ++e) {
+          u[e] = fmul2(z[j][e], bf16x2_to_f2(w[e]));
+          amax = fmaxf(amax, fmaxf(fabsf(lo_f(u[e])), fabsf(hi_f(u[e]))));
         }
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        const float sc = group_scale(amax);
-        if (active) {
-          const float r = __frcp_rn(sc);
+        const float su = amax_div_448(amax);
+        float as = __fmul_rn(su, rs), div = su, mul = 1.0f;
+        if (!(as >= 1e-12f)) {
+          as = div = 1e-12f;
+          mul = rs;
+        }
+        if (c < nch && ok) {
+          const float nr = -__frcp_rn(div);
+          const uint64_t d2 = pack_f2(div, div), nr2 = pack_f2(nr, nr), m2 = pack_f2(mul, mul);
           uint32_t q[2];
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            q[h] = f2_to_e4m3x2(div_by_scale(z[j][4 * h], sc, r), div_by_scale(z[j][4 * h + 1], sc, r)) |
-                   (f2_to_e4m3x2(div_by_scale(z[j][4 * h + 2], sc, r), div_by_scale(z[j][4 * h + 3], sc, r)) << 16);
+          for (int h = 0; h < 2; ++h) {
+            const uint64_t q0 = neg_div_by_scale2(fmul2(u[2 * h], m2), d2, nr2);
+            const uint64_t q1 = neg_div_by_scale2(fmul2(u[2 * h + 1], m2), d2, nr2);
+            q[h] = (f2_to_e4m3x2(lo_f(q0), hi_f(q0)) | (f2_to_e4m3x2(lo_f(q1), hi_f(q1)) << 16)) ^ 0x80808080u;
+          }
           *reinterpret_cast<uint2*>(p.A + static_cast<size_t>(row) * p.H + c * 8) = make_uint2(q[0], q[1]);
-          if ((lane & 15) == 0) p.As[static_cast<size_t>(row) * (p.H / 128) + c / 16] = sc;
+          if ((lane & 15) == 0) p.As[static_cast<size_t>(row) * (p.H / 128) + c / 16] = as;
         }
       }
     }

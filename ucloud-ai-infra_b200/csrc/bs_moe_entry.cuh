@@ -141,14 +141,24 @@ bs::GroupedParams grouped_params(const void* A, const float* As, const float* Bs
   return p;
 }
 
-template <int C>
-int launch_block(const bs::BlockParams& p, bool wide, int threads, int num_sms, cudaStream_t s) {
-  auto kern = wide ? bs::k_block_norm<C, true> : bs::k_block_norm<C, false>;
+template <int C, bool WIDE>
+int launch_block(const bs::BlockParams& p, int threads, int num_sms, cudaStream_t s) {
+  constexpr auto kern = bs::k_block_norm<C, WIDE>;
+  const int rc = prepare_kernel<kern>(bs::kBlockRingBytes, 0);
+  if (rc != BS_OK) return rc;
+  const int rows = bs::block_stage_rows(p.weights ? p.k : 1, p.H);
+  const int smem = bs::block_stages(rows, p.H) * rows * 2 * p.H;
   int per_sm = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, 0) != cudaSuccess || per_sm < 1) per_sm = 1;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads + 32, smem) != cudaSuccess || per_sm < 1)
+    per_sm = 1;
   cudaGetLastError();
   const int grid = p.T < per_sm * num_sms ? p.T : per_sm * num_sms;
-  return launch_pdl(kern, grid, threads, 0, s, "k_block_norm launch", p);
+  return launch_pdl(kern, grid, threads + 32, smem, s, "k_block_norm launch", p);
+}
+
+template <int C>
+int launch_block_c(const bs::BlockParams& p, bool wide, int threads, int num_sms, cudaStream_t s) {
+  return wide ? launch_block<C, true>(p, threads, num_sms, s) : launch_block<C, false>(p, threads, num_sms, s);
 }
 
 }  // namespace
@@ -238,13 +248,13 @@ int bs_fp8_block_norm_quant(const void* y, long long ldy, int rows_y, const floa
                             const void* post_weight, const void* gate, int gate_kind, long long ldg, float scale,
                             float residual_scale, const void* pre_weight, float eps, void* A, float* As, int T, int H,
                             void* stream) {
-  if (T < 0 || H <= 0 || H % 128 || H > bs::kBlockMaxThreads * bs::kBlockMaxChunks * 8) return BS_ERR_ARG;
+  if (T < 0 || H <= 0 || H % 128 || H > bs::kBlockMaxH) return BS_ERR_ARG;
   if (wide != 0 && wide != 1) return BS_ERR_ARG;
   const int per16 = wide ? 4 : 8;  // elements of the residual per 16 bytes
   if (ldy < H || ldy % 8 || ldr < H || ldr % per16 || ldo < H || ldo % per16 || rows_y < 0) return BS_ERR_ARG;
   if (!(eps >= 0.f) || gate_kind < 0 || gate_kind > 3 || (gate_kind != 0) != (gate != nullptr)) return BS_ERR_ARG;
   if ((gate_kind == 3 && (ldg < H || ldg % 8)) || (gate_kind == 2 && ldg < 1)) return BS_ERR_ARG;
-  if ((weights == nullptr) != (slot_row == nullptr) || (weights && top_k <= 0) || (!weights && rows_y < T)) return BS_ERR_ARG;
+  if ((weights == nullptr) != (slot_row == nullptr) || (weights && (top_k <= 0 || top_k > bs::kMaxTopK)) || (!weights && rows_y < T)) return BS_ERR_ARG;
   if (T == 0) return BS_OK;
   if (!y || !residual || !out || (pre_weight && (!A || !As))) return BS_ERR_ARG;
   if (!aligned16(y) || !aligned16(residual) || !aligned16(out) || !aligned16(post_weight) || !aligned16(pre_weight) ||
@@ -271,17 +281,22 @@ int bs_fp8_block_norm_quant(const void* y, long long ldy, int rows_y, const floa
   p.residual_scale = residual_scale;
   p.pre = static_cast<const __nv_bfloat16*>(pre_weight);
   p.eps = eps;
+  p.inv_h = 1.0f / static_cast<float>(H);
   p.A = static_cast<uint8_t*>(A);
   p.As = As;
   p.T = T;
   p.H = H;
   const int chunks = H / 8;
-  const int c = chunks <= bs::kBlockMaxThreads ? 1 : chunks <= 2 * bs::kBlockMaxThreads ? 2 : 4;
+  const int c = chunks <= bs::kBlockMaxThreads ? 1 : chunks <= 2 * bs::kBlockMaxThreads ? 2 : chunks <= 4 * bs::kBlockMaxThreads ? 4 : 7;
   const int threads = ((chunks + c - 1) / c + 31) / 32 * 32;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (c == 1) return launch_block<1>(p, wide != 0, threads, d->num_sms, s);
-  if (c == 2) return launch_block<2>(p, wide != 0, threads, d->num_sms, s);
-  return launch_block<4>(p, wide != 0, threads, d->num_sms, s);
+  p.status = d->status;
+  switch (c) {
+    case 1: return launch_block_c<1>(p, wide != 0, threads, d->num_sms, s);
+    case 2: return launch_block_c<2>(p, wide != 0, threads, d->num_sms, s);
+    case 4: return launch_block_c<4>(p, wide != 0, threads, d->num_sms, s);
+    default: return launch_block_c<7>(p, wide != 0, threads, d->num_sms, s);
+  }
 }
 
 }  // extern "C"
