@@ -197,15 +197,15 @@ int bs_fp8_grouped_gemm_silu_quant(const void* A, const void* B, void* Q, const 
  *   n = z / sqrt(mean(z^2) + eps) * post_weight   (post_weight NULL: n = z)
  *   h = residual_scale * residual[t] + scale * gate * n
  *   v = h / sqrt(mean(h^2) + eps) * pre_weight, from the unrounded h; then A, As as bs_fp8_group_quant without a
- *       rounding of v to bf16 before it   (pre_weight NULL: no A, As)
- * residual and out are bf16 (wide = 0) or fp32 (1), row strides ldr and ldo; out may be residual. gate_kind 0 none
+ *       rounding of v to bf16 before it, and V [T, H] = bf16(v) where V is not NULL   (pre_weight NULL: none of them)
+ * top_k <= 32. residual may be NULL (h = scale * gate * n). residual and out are bf16 (wide = 0) or fp32 (1), row strides ldr and ldo; out may be residual. gate_kind 0 none
  * (1), 1 per channel [H], 2 per token (row stride ldg), 3 per element (row stride ldg); bf16. H: a multiple of
  * 128, at most 16384; pointers (but a per-token gate's) and row strides in whole 16 bytes. */
 int bs_fp8_block_norm_quant(const void* y, long long ldy, int rows_y, const float* weights, const int* slot_row,
                             int top_k, const void* residual, long long ldr, void* out, long long ldo, int wide,
                             const void* post_weight, const void* gate, int gate_kind, long long ldg, float scale,
-                            float residual_scale, const void* pre_weight, float eps, void* A, float* As, int T, int H,
-                            void* stream);
+                            float residual_scale, const void* pre_weight, float eps, void* A, float* As, void* V, int T,
+                            int H, void* stream);
 
 /* Reads the device status word of the current device (synchronises the device). Writes the
  * code to *code and clears it when `clear` is non-zero. Counterpart of the reference's

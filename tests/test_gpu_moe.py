@@ -263,6 +263,20 @@ def test_block_plain_add_and_norm(cuda_lib, k):
     _check_block(got, M.block(y, res, pre=pre, weights=w, slot_row=slot), False)
 
 
+@pytest.mark.parametrize("k", [0, 3])
+def test_block_without_residual_and_norm_out(cuda_lib, k):
+    """h = scale * gate * n alone, and the bf16 norm beside its group quant."""
+    y, res, post, pre, w, slot, g = _block_case(33, 768, k, False, 12)
+    gt = torch.sigmoid(torch.randn(768, generator=g)).to(torch.bfloat16)
+    h, A, As, v = _ops().block_norm_quant(y.cuda(), None, post_weight=post.cuda(), gate=gt.cuda(), scale=1.5,
+                                          pre_weight=pre.cuda(), route=_route_of(w, slot), norm_out=True)
+    want = M.block(y, torch.zeros_like(res), post=post, gate=gt, scale=1.5, pre=pre, weights=w, slot_row=slot)
+    _check_block((h, A, As), want, False)
+    _within(v, want[2], want[3], BF16_HALF)
+    got = _ops().block_norm_quant(y.cuda(), None, route=_route_of(w, slot))
+    _check_block(got, M.block(y, torch.zeros_like(res), weights=w, slot_row=slot), False)
+
+
 def test_block_strides_and_zero_rows(cuda_lib):
     """Rows of wider tensors, odd starts (copied), a broadcast gate per token, all-zero rows, T = 0."""
     y, res, post, pre, _, _, g = _block_case(9, 384, 0, False, 6)
@@ -330,6 +344,58 @@ def test_side_stream_and_graph(cuda_lib):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a.float(), b.float()) for a, b in zip(out, w))
+
+
+def _experts(E, inter, H, seed):
+    w13, s13 = zip(*[O.make_weight(2 * inter, H, seed + e) for e in range(E)])
+    w2, s2 = zip(*[O.make_weight(H, inter, seed + 100 + e) for e in range(E)])
+    stack = lambda ws: torch.stack([t.view(torch.uint8) for t in ws]).view(torch.float8_e4m3fn)  # noqa: E731
+    return stack(w13), torch.stack(s13), stack(w2), torch.stack(s2)
+
+
+@pytest.mark.parametrize("T", [1, 90])
+def test_sparse_block(cuda_lib, monkeypatch, T):
+    """The path that runs them together: two SparseBlocks, tile-first after post_load. Each stage is checked against the
+    64-bit oracle on the stage's own inputs, expert halves on two ranks add up to the whole."""
+    import fp8_hand_b200.fp8_hand_sm100 as hand
+    from fp8_hand_b200 import sglang_compat as S
+    monkeypatch.setattr(hand, "ENABLED", True)
+    ops = _ops()
+    E, k, H, inter = 6, 2, 512, 256
+    w13, s13, w2, s2 = _experts(E, inter, H, 40)
+    g = torch.Generator().manual_seed(T)
+    bf = torch.bfloat16
+    norms = [(1 + 0.1 * torch.randn(H, generator=g)).to(bf) for _ in range(4)]
+    router = torch.randn(E, H, generator=g).to(bf)
+    mlp = S.SparseMLP(w13.cuda(), s13.cuda(), w2.cuda(), s2.cuda(), k)
+    block = S.SparseBlock(router.cuda(), mlp, norms[1].cuda(), post_norm=norms[2].cuda(), scale=0.5).cuda()
+    x = torch.randn(T, H, generator=g).to(bf)
+    state = S.SparseBlock.enter(x.cuda(), norms[0].cuda())
+    row_major = block(*state)
+    S.post_load(block)
+    assert mlp.w13_weight.device.type == "meta" and mlp.w13_weight.tiles.shape == (E, 2 * inter // 128, H // 128, 128, 128)
+    out = block(*state)
+    assert all(torch.equal(a.float(), b.float()) for a, b in zip(out, row_major))
+    # stage by stage
+    h, A, As, v = state
+    logits = torch.nn.functional.linear(v, router.cuda())
+    rows, route = mlp.experts((A, As), logits)
+    _check_route(route, logits.cpu(), k)
+    off, src, _ = M.plan(route.ids.cpu(), 0, E)
+    Q, Qs = ops.grouped_gemm_silu_quant(A, mlp.w13_weight.tiles, As, s13.cuda(), route, b_tiled=True)
+    M.check_quant(Q.cpu(), Qs.cpu(), *M.silu_mul(*M.grouped(A.cpu(), As.cpu(), w13, s13, off, src)), 1e-10 / 448)
+    _within(rows, *M.grouped(Q.cpu(), Qs.cpu(), w2, s2, off, torch.arange(T * k)), BF16_HALF)
+    want = M.block(rows.cpu(), h.cpu(), post=norms[2], scale=0.5, pre=norms[1], weights=route.weights.cpu(),
+                   slot_row=route.slot_row.cpu())
+    _check_block(out[:3], want, False)
+    block(*out)  # the stream goes on
+    # two expert-parallel halves
+    whole = mlp((A, As), logits)
+    parts = [S.SparseMLP(w13[i:i + 3].cuda(), s13[i:i + 3].cuda(), w2[i:i + 3].cuda(), s2[i:i + 3].cuda(), k, first_expert=i)
+             ((A, As), logits) for i in (0, 3)]
+    # each half and the whole are rounded once to bf16
+    lim = 2.0 ** -8 * 1.01 * (parts[0].abs() + parts[1].abs() + whole.abs()).double().cpu() + 1e-30
+    assert bool(((parts[0].double() + parts[1].double() - whole.double()).abs().cpu() <= lim + 1e-6 * lim.max()).all())
 
 
 def test_refusals(cuda_lib):

@@ -60,7 +60,7 @@ def test_grouped_arguments(lib):
 
 def test_block_arguments(lib):
     ok = dict(y=P, ldy=256, rows=4, w=None, sr=None, k=0, res=P, ldr=256, out=P, ldo=256, wide=0, post=None, gate=None, kind=0,
-              ldg=0, scale=1.0, rscale=1.0, pre=P, eps=1e-6, A=P, As=P, T=4, H=256)
+              ldg=0, scale=1.0, rscale=1.0, pre=P, eps=1e-6, A=P, As=P, V=None, T=4, H=256)
 
     def call(**kw):
         return lib.bs_fp8_block_norm_quant(*{**ok, **kw}.values(), None)
@@ -68,7 +68,7 @@ def test_block_arguments(lib):
     for bad in (dict(H=200), dict(H=16512, ldy=16512, ldr=16512, ldo=16512), dict(ldy=128), dict(ldy=260), dict(ldr=258),
                 dict(ldo=250), dict(wide=2), dict(eps=-1.0), dict(eps=float("nan")), dict(kind=1), dict(gate=P), dict(kind=4, gate=P),
                 dict(kind=3, gate=P, ldg=128), dict(kind=2, gate=P, ldg=0), dict(w=P), dict(w=P, sr=P), dict(rows=3), dict(T=-1),
-                dict(A=None), dict(res=None)):
+                dict(A=None), dict(V=P, pre=None), dict(w=P, sr=P, k=33)):
         assert call(**bad) == 1, bad
     assert call(y=P + 2) == 2 and call(pre=P + 8) == 2 and call(kind=1, gate=P + 2) == 2
     assert call(T=0, rows=0) == 0

@@ -2,11 +2,11 @@
 //   z   = y[t]                                             (dense block output)
 //       = sum_s weights[t, s] * y[slot_row[t, s]]          (experts' rows; slots with row -1 add nothing)
 //   n   = z * (1 / sqrt(mean(z^2) + eps)) * post           (norm after the block; optional)
-//   h   = residual_scale * residual + scale * gate * n     (gate per channel, token or element; optional)
+//   h   = residual_scale * residual + scale * gate * n     (residual, and gate per channel, token or element: optional)
 //   v   = h * (1 / sqrt(mean(h^2) + eps)) * pre            (norm before the next block)
 //   As  = max(amax(v over 128) / 448, 1e-12),  A = e4m3_rn(v / As)
 // Every step is fp32; h is rounded once to the residual's type when it is stored, and v is taken from the unrounded
-// h and goes to e4m3 without a rounding to bf16 between.
+// h and goes to e4m3 without a rounding to bf16 between (V, if asked for, is bf16_rn(v): a router's input).
 //
 // Bound: HBM. Per token k (or 1) rows of bf16 and the residual are read, the residual and the e4m3 row written; what
 // costs is keeping enough of those reads in flight beside two reductions per row, in few instructions per element. A
@@ -34,7 +34,7 @@ struct BlockParams {
   const float* weights;      // [T, k]; nullptr: dense
   const int* slot_row;       // [T, k]
   int k;
-  const void* residual;      // [T, ldr] bf16 or fp32
+  const void* residual;      // [T, ldr] bf16 or fp32; nullptr: none
   long long ldr;
   void* out;                 // [T, ldo] of the residual's type; may be the residual itself
   long long ldo;
@@ -47,6 +47,7 @@ struct BlockParams {
   float eps, inv_h;          // inv_h: 1 / H
   uint8_t* A;                // [T, H]
   float* As;                 // [T, H / 128]
+  __nv_bfloat16* V;          // [T, H] or nullptr
   int T, H;
   int* status;
 };
@@ -203,7 +204,9 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
     for (int j = 0; j < C; ++j) {
       const int c = t + nt * j;
       if (c < nch) {
-        if constexpr (WIDE) {
+        if (!p.residual) {
+          res[j][0] = res[j][WIDE ? 1 : 0] = make_uint4(0, 0, 0, 0);
+        } else if constexpr (WIDE) {
           const uint4* rr = reinterpret_cast<const uint4*>(static_cast<const float*>(p.residual) + row * p.ldr + c * 8);
           res[j][0] = rr[0];
           res[j][1] = rr[1];
@@ -347,6 +350,16 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
           }
           *reinterpret_cast<uint2*>(p.A + static_cast<size_t>(row) * p.H + c * 8) = make_uint2(q[0], q[1]);
           if ((lane & 15) == 0) p.As[static_cast<size_t>(row) * (p.H / 128) + c / 16] = as;
+          if (p.V) {
+            const uint64_t rs2 = pack_f2(rs, rs);
+            uint32_t v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint64_t x = fmul2(u[e], rs2);
+              v[e] = pack_bf16x2(lo_f(x), hi_f(x));
+            }
+            *reinterpret_cast<uint4*>(p.V + static_cast<size_t>(row) * p.H + c * 8) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
         }
       }
     }

@@ -246,19 +246,19 @@ int bs_fp8_grouped_gemm_silu_quant(const void* A, const void* B, void* Q, const 
 int bs_fp8_block_norm_quant(const void* y, long long ldy, int rows_y, const float* weights, const int* slot_row,
                             int top_k, const void* residual, long long ldr, void* out, long long ldo, int wide,
                             const void* post_weight, const void* gate, int gate_kind, long long ldg, float scale,
-                            float residual_scale, const void* pre_weight, float eps, void* A, float* As, int T, int H,
-                            void* stream) {
+                            float residual_scale, const void* pre_weight, float eps, void* A, float* As, void* V, int T,
+                            int H, void* stream) {
   if (T < 0 || H <= 0 || H % 128 || H > bs::kBlockMaxH) return BS_ERR_ARG;
   if (wide != 0 && wide != 1) return BS_ERR_ARG;
   const int per16 = wide ? 4 : 8;  // elements of the residual per 16 bytes
-  if (ldy < H || ldy % 8 || ldr < H || ldr % per16 || ldo < H || ldo % per16 || rows_y < 0) return BS_ERR_ARG;
+  if (ldy < H || ldy % 8 || (residual && (ldr < H || ldr % per16)) || ldo < H || ldo % per16 || rows_y < 0) return BS_ERR_ARG;
   if (!(eps >= 0.f) || gate_kind < 0 || gate_kind > 3 || (gate_kind != 0) != (gate != nullptr)) return BS_ERR_ARG;
   if ((gate_kind == 3 && (ldg < H || ldg % 8)) || (gate_kind == 2 && ldg < 1)) return BS_ERR_ARG;
   if ((weights == nullptr) != (slot_row == nullptr) || (weights && (top_k <= 0 || top_k > bs::kMaxTopK)) || (!weights && rows_y < T)) return BS_ERR_ARG;
   if (T == 0) return BS_OK;
-  if (!y || !residual || !out || (pre_weight && (!A || !As))) return BS_ERR_ARG;
+  if (!y || !out || (pre_weight && (!A || !As)) || (V && !pre_weight)) return BS_ERR_ARG;
   if (!aligned16(y) || !aligned16(residual) || !aligned16(out) || !aligned16(post_weight) || !aligned16(pre_weight) ||
-      !aligned16(A) || (gate_kind != 2 && !aligned16(gate)))
+      !aligned16(A) || !aligned16(V) || (gate_kind != 2 && !aligned16(gate)))
     return BS_ERR_ALIGN;
   DeviceState* d = device_state();
   if (!d) return BS_ERR_CUDA;
@@ -284,6 +284,7 @@ int bs_fp8_block_norm_quant(const void* y, long long ldy, int rows_y, const floa
   p.inv_h = 1.0f / static_cast<float>(H);
   p.A = static_cast<uint8_t*>(A);
   p.As = As;
+  p.V = static_cast<__nv_bfloat16*>(V);
   p.T = T;
   p.H = H;
   const int chunks = H / 8;

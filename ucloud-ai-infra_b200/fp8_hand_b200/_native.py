@@ -44,7 +44,7 @@ SIGNATURES = {
     "bs_fp8_grouped_gemm": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _I, _I, _VP]),
     "bs_fp8_grouped_gemm_silu_quant": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _VP]),
     "bs_fp8_block_norm_quant": (_I, [_VP, _LL, _I, _VP, _VP, _I, _VP, _LL, _VP, _LL, _I, _VP, _VP, _I, _LL, _F, _F,
-                                     _VP, _F, _VP, _VP, _I, _I, _VP]),
+                                     _VP, _F, _VP, _VP, _VP, _I, _I, _VP]),
     "bs_fp8_status": (_I, [ctypes.POINTER(_I), _I]),
     "bs_fp8_selftest_wait_timeout": (_I, [_U64, _VP]),
     "bs_fp8_launch_plan": (_I, [_I, _I, _I, _I, ctypes.POINTER(_I), _I]),

@@ -8,7 +8,7 @@ import this module instead:
                                           SGLANG_FP8_HAND_FUSED_MIN_M (H:41-43)
   select(N, M) -> dict                    tile choice of an M x N product (H:74-81)
   precompile() -> list[str]               build step, never on the request path (H:596-611)
-  relayout(model, cache=None)             tile-first weight pre-pack after loading (H:652-672); with a
+  relayout(model, cache=None)             tile-first weight pre-pack after loading (H:652-672), expert weights included; with a
                                           cache file (tilepack.py) the packed tiles are read, not permuted
   fused_gate_up(proj, x) -> (Q, Qs)|None  fused MLP front half (H:675-701)
   matmul(A, B, C, As, Bs, M, N, K, block_size) -> bool   GEMM hook (H:704-719)
@@ -133,8 +133,34 @@ def relayout(model: torch.nn.Module, cache: str | os.PathLike | None = None) -> 
         module.weight.tiles = tiles
     if cache is not None and stored is None and packed:
         tilepack.save(cache, packed)
+    relayout_experts(model)
     torch.cuda.empty_cache()
     logger.info("FP8 hand: %d linears tile first (%d from %s)", len(todo), len(todo) - len(packed), cache)
+
+
+EXPERT_WEIGHTS = ("w13_weight", "w2_weight")  # SGLang's FusedMoE parameter names, each with <name>_scale_inv
+
+
+def relayout_experts(model: torch.nn.Module) -> int:
+    """The expert weights of every mixture-of-experts module (e4m3 [E, N, K] with fp32 block scales [E, N/128, K/128]) to
+    tile-first storage [E, N/128, K/128, 128, 128]; returns how many were moved. Called by relayout."""
+    moved = 0
+    for module in model.modules():
+        for name in EXPERT_WEIGHTS:
+            weight, scale = getattr(module, name, None), getattr(module, name + "_scale_inv", None)
+            if weight is None or scale is None or getattr(weight, "tiles", None) is not None:
+                continue
+            if weight.dim() != 3 or weight.dtype != torch.float8_e4m3fn or weight.shape[1] % BK or weight.shape[2] % BK:
+                continue
+            E, N, K = weight.shape
+            if tuple(scale.shape) != (E, N // BK, K // BK):
+                continue
+            tiles = ops.pack_tiles(weight.data.reshape(E * N, K)).view(E, N // BK, K // BK, BK, BK)
+            setattr(module, name, Parameter(torch.empty(E, N, K, dtype=torch.float8_e4m3fn, device="meta"),
+                                            requires_grad=False))
+            getattr(module, name).tiles = tiles
+            moved += 1
+    return moved
 
 
 def fused_gate_up(proj, x):

@@ -445,42 +445,51 @@ def _norm_weight(w: torch.Tensor | None, H: int, index: int) -> int | None:
     return w.data_ptr()
 
 
-def block_norm_quant(y: torch.Tensor, residual: torch.Tensor, *, post_weight: torch.Tensor | None = None,
+def block_norm_quant(y: torch.Tensor, residual: torch.Tensor | None, *, post_weight: torch.Tensor | None = None,
                      gate: torch.Tensor | None = None, scale: float = 1.0, residual_scale: float = 1.0,
                      pre_weight: torch.Tensor | None = None, eps: float = 1e-6, route: MoeRoute | None = None,
-                     out: torch.Tensor | None = None):
+                     out: torch.Tensor | None = None, norm_out: bool = False):
     """The end of a block and the start of the next one, in one pass and in fp32:
       z = y, or with `route` the experts' rows summed per token, sum_s weights[t, s] * y[slot_row[t, s]]
       n = rmsnorm(z) * post_weight                     (post_weight None: n = z)
       h = residual_scale * residual + scale * gate * n
       A, As = group_quant(rmsnorm(h) * pre_weight)     (pre_weight None: not made)
-    y bf16 [T, H] (or [rows, H] with `route`), residual bf16 or fp32 [T, H], gate bf16 [H], [T, 1] or [T, H]. h is
-    rounded once, into `out` (a new tensor like residual; pass out=residual to update it in place); A is
-    taken from the unrounded h. Returns (h, A e4m3 [T, H], As fp32 [T, H/128]), or h alone without pre_weight."""
+    y bf16 [T, H] (or [rows, H] with `route`), residual bf16 or fp32 [T, H] (None: h = scale * gate * n, bf16), gate
+    bf16 [H], [T, 1] or [T, H]. h is rounded once, into `out` (a new tensor like residual; pass out=residual to update
+    it in place); A is taken from the unrounded h. Returns (h, A e4m3 [T, H], As fp32 [T, H/128]), with norm_out also
+    the norm itself in bf16 (a router's input), or h alone without pre_weight."""
     bf16 = torch.bfloat16
-    wide = residual.dtype == torch.float32
     if y.dim() != 2 or y.dtype != bf16:
         raise ValueError("y must be bf16 [rows, H]")
-    if residual.dim() != 2 or not (wide or residual.dtype == bf16):
-        raise ValueError("residual must be bf16 or fp32 [T, H]")
-    index, dev = _one_device(y, residual), y.device
-    T, H = residual.shape
     rows_y, hy = y.shape
+    if residual is None:
+        wide, index, H = False, _one_device(y), hy
+        T = rows_y if route is None else route.slot_row.shape[0]
+    else:
+        wide = residual.dtype == torch.float32
+        if residual.dim() != 2 or not (wide or residual.dtype == bf16):
+            raise ValueError("residual must be bf16 or fp32 [T, H]")
+        index = _one_device(y, residual)
+        T, H = residual.shape
+    dev, h_type = y.device, torch.float32 if wide else bf16
     if H % BLOCK or not 0 < H <= 16384:
         raise ValueError("H must be a multiple of 128, at most 16384")
     if hy != H or (route is None and rows_y != T):
         raise ValueError("y must have residual's shape (or be a route's rows)")
     given = out
     if out is None:
-        out, ldo = torch.empty((T, H), dtype=residual.dtype, device=dev), H
+        out, ldo = torch.empty((T, H), dtype=h_type, device=dev), H
     else:
-        if out.shape != (T, H) or out.dtype != residual.dtype or out.get_device() != index:
+        if out.shape != (T, H) or out.dtype != h_type or out.get_device() != index:
             raise ValueError("out must be like residual")
         same, ldo = _rows16(out)
         if same is not out:
             raise ValueError("out must have contiguous 16-byte aligned rows")
     y, ldy = _rows16(y)
-    residual, ldr = (out, ldo) if residual is given else _rows16(residual)
+    r_ptr, ldr = None, 0
+    if residual is not None:
+        residual, ldr = (out, ldo) if residual is given else _rows16(residual)
+        r_ptr = residual.data_ptr()
     post, pre = _norm_weight(post_weight, H, index), _norm_weight(pre_weight, H, index)
     kind, ldg, g_ptr = 0, 0, None
     if gate is not None:
@@ -510,12 +519,19 @@ def block_norm_quant(y: torch.Tensor, residual: torch.Tensor, *, post_weight: to
         if w.dtype != torch.float32 or rows.dtype != torch.int32 or not (w.is_contiguous() and rows.is_contiguous()):
             raise ValueError("the route's weights and rows must be contiguous fp32 and int32")
         w_ptr, s_ptr, k = w.data_ptr(), rows.data_ptr(), rows.shape[1]
-    A = As = a_ptr = as_ptr = None
+    A = As = V = a_ptr = as_ptr = v_ptr = None
     if pre is not None:
         A = torch.empty((T, H), dtype=E4M3, device=dev)
         As = torch.empty((T, H // BLOCK), dtype=torch.float32, device=dev)
         a_ptr, as_ptr = A.data_ptr(), As.data_ptr()
+        if norm_out:
+            V = torch.empty((T, H), dtype=bf16, device=dev)
+            v_ptr = V.data_ptr()
+    elif norm_out:
+        raise ValueError("norm_out needs pre_weight")
     _native.call(_native.lib().bs_fp8_block_norm_quant, "bs_fp8_block_norm_quant", index, y.data_ptr(), ldy, rows_y, w_ptr,
-                 s_ptr, k, residual.data_ptr(), ldr, out.data_ptr(), ldo, wide, post, g_ptr, kind, ldg, scale,
-                 residual_scale, pre, eps, a_ptr, as_ptr, T, H)
-    return out if pre is None else (out, A, As)
+                 s_ptr, k, r_ptr, ldr, out.data_ptr(), ldo, wide, post, g_ptr, kind, ldg, scale,
+                 residual_scale, pre, eps, a_ptr, as_ptr, v_ptr, T, H)
+    if pre is None:
+        return out
+    return (out, A, As, V) if norm_out else (out, A, As)

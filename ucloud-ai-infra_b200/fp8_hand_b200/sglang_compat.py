@@ -11,6 +11,11 @@ drop-in module is exercised exactly as SGLang would call it:
       the fused output reaches down_proj (:50-53).
   GatedMLP.forward(x)                                             the patched MLP forward (:45-56).
   post_load(model)                                                the loader hook (:59-65).
+
+The same block as a mixture of experts, for which the reference has no counterpart (its models are dense):
+
+  SparseMLP            the expert weights under the parameter names of SGLang's FusedMoE; routed products and their sum
+  SparseBlock          norm -> router -> experts -> norm, gate and residual, handing the next block its quantised input
 """
 from __future__ import annotations
 
@@ -86,6 +91,73 @@ class GatedMLP(nn.Module):
         gate_up, _ = self.gate_up_proj(x)
         x, _ = self.down_proj(silu_and_mul(gate_up))
         return x
+
+
+class SparseMLP(nn.Module):
+    """Gated MLP as a mixture of block-FP8 experts, under the parameter names of SGLang's FusedMoE:
+    w13_weight e4m3 [E, 2I, H] (gate rows, then up rows) with w13_weight_scale_inv fp32 [E, 2I/128, H/128], and
+    w2_weight e4m3 [E, H, I] with w2_weight_scale_inv. After post_load the weights are tile-first (their parameters stay
+    on the meta device and carry `.tiles`). E are the experts held here, numbers first_expert .. first_expert + E - 1
+    of the router's (expert parallelism: the ranks' outputs add up)."""
+
+    def __init__(self, w13_weight: torch.Tensor, w13_weight_scale_inv: torch.Tensor, w2_weight: torch.Tensor,
+                 w2_weight_scale_inv: torch.Tensor, top_k: int, *, renormalize: bool = True, routed_scale: float = 1.0,
+                 first_expert: int = 0):
+        super().__init__()
+        self.w13_weight = nn.Parameter(w13_weight, requires_grad=False)
+        self.w13_weight_scale_inv = nn.Parameter(w13_weight_scale_inv, requires_grad=False)
+        self.w2_weight = nn.Parameter(w2_weight, requires_grad=False)
+        self.w2_weight_scale_inv = nn.Parameter(w2_weight_scale_inv, requires_grad=False)
+        self.top_k, self.renormalize, self.routed_scale = top_k, renormalize, routed_scale
+        self.first_expert = first_expert
+
+    def experts(self, x, router_logits: torch.Tensor) -> tuple[torch.Tensor, ops.MoeRoute]:
+        """x bf16 [T, H] or its group quant (A, As) -> (the experts' rows bf16 [T * top_k, H], the route)."""
+        A, As = x if isinstance(x, tuple) else ops.group_quant(x, BLOCK)
+        route = ops.moe_route(router_logits, self.top_k, renormalize=self.renormalize, scale=self.routed_scale,
+                              experts=(self.first_expert, self.w13_weight.shape[0]))
+        w13, w2 = (getattr(w, "tiles", None) for w in (self.w13_weight, self.w2_weight))
+        q, s = ops.grouped_gemm_silu_quant(A, self.w13_weight if w13 is None else w13, As, self.w13_weight_scale_inv, route,
+                                           b_tiled=w13 is not None)
+        rows = ops.grouped_gemm(q, self.w2_weight if w2 is None else w2, s, self.w2_weight_scale_inv, route,
+                                b_tiled=w2 is not None)
+        return rows, route
+
+    def forward(self, x, router_logits: torch.Tensor) -> torch.Tensor:
+        """sum over a token's slots of weight * expert(x): bf16 [T, H]."""
+        rows, route = self.experts(x, router_logits)
+        return ops.block_norm_quant(rows, None, route=route)
+
+
+class SparseBlock(nn.Module):
+    """A mixture-of-experts block between its norms. The stream between blocks is (h, A, As, v): the residual, the group
+    quant of its norm (the experts' input) and the norm in bf16 (the router's). One call takes this block's
+    (h, A, As, v) to the next's, whose norm weight is next_norm:
+      h' = residual_scale * h + scale * gate * rmsnorm(experts(A, As; router(v))) * post_norm"""
+
+    def __init__(self, router_weight: torch.Tensor, mlp: SparseMLP, next_norm: torch.Tensor,
+                 post_norm: torch.Tensor | None = None, gate: torch.Tensor | None = None, scale: float = 1.0,
+                 residual_scale: float = 1.0, eps: float = 1e-6):
+        super().__init__()
+        self.router_weight = nn.Parameter(router_weight, requires_grad=False)
+        self.mlp = mlp
+        self.next_norm = nn.Parameter(next_norm, requires_grad=False)
+        self.post_norm = None if post_norm is None else nn.Parameter(post_norm, requires_grad=False)
+        self.gate = None if gate is None else nn.Parameter(gate, requires_grad=False)
+        self.scale, self.residual_scale, self.eps = scale, residual_scale, eps
+
+    @staticmethod
+    def enter(x: torch.Tensor, norm: torch.Tensor, eps: float = 1e-6):
+        """(h, A, As, v) of a stack's first block from the embeddings x bf16 [T, H]."""
+        _, A, As, v = ops.block_norm_quant(x, None, pre_weight=norm, eps=eps, norm_out=True)
+        return x, A, As, v
+
+    def forward(self, h, A, As, v):
+        logits = nn.functional.linear(v, self.router_weight)
+        rows, route = self.mlp.experts((A, As), logits)
+        return ops.block_norm_quant(rows, h, post_weight=self.post_norm, gate=self.gate, scale=self.scale,
+                                    residual_scale=self.residual_scale, pre_weight=self.next_norm, eps=self.eps,
+                                    route=route, norm_out=True)
 
 
 def post_load(model: nn.Module, cache=None) -> None:
