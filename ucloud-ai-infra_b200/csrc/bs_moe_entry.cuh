@@ -4,10 +4,11 @@
 
 namespace {
 
-// Tokens per CTA of the route kernels: one round of a CTA's warps, more when that would take more CTAs than SMs
-// (k_moe_place reads every CTA's counts).
+// Tokens per CTA of the route kernels: one round of a CTA's warps, more when that would take more CTAs than fit on the
+// device at once, two per SM (k_moe_place reads every CTA's counts).
 int route_tokens_per_cta(int T, int num_sms) {
-  const int rounds = (T + bs::kRouteFuse * num_sms - 1) / (bs::kRouteFuse * num_sms);
+  const int at_once = bs::kRouteFuse * 2 * num_sms;
+  const int rounds = T / at_once + (T % at_once != 0);
   return bs::kRouteFuse * (rounds > 1 ? rounds : 1);
 }
 int route_grid(int T, int num_sms) {
