@@ -138,15 +138,19 @@ __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wai
 // load would put them (chunk c of row r at chunk c ^ (r % 8)). A gathering TMA load (four rows each) was measured first
 // and is the bound of the kernel there: 8192 tokens x 8 of 64 experts, K = 5120, N = 2048, one product: 1894 us gathered
 // by TMA, 843 us with the rows already in order.
-template <bool FUSED>
+// BOX (plain bf16 output): whole 32-row pieces of a tile leave by TMA from 64 KB of shared memory, at three stages. Measured
+// (64 experts, K = 1024, N = 5120; without and with): mean 30 rows per expert 68 and 75 us, 125 rows 102 and 102, 1024
+// rows 516 and 493.
+template <bool FUSED, bool BOX>
 struct GroupedRowsCfg {
   using Regs = RegSplit<384, 168, 40, 232>;
   static constexpr int kThreads = Regs::kThreads;
-  static constexpr int kStages = 4;
+  static constexpr int kStages = BOX ? 3 : 4;
   static constexpr int kABytes = 128 * 128;
   static constexpr int kStageBytes = kABytes + 256 * 128;
   static constexpr int kXchOff = kStages * kStageBytes;
-  static constexpr int kXchBytes = FUSED ? 128 * 2 * 4 : 8 * 2048;  // amax halves; plain: 2 KB per promotion warp
+  // amax halves; plain: 2 or 8 KB per promotion warp
+  static constexpr int kXchBytes = FUSED ? 128 * 2 * 4 : BOX ? 8 * 8192 : 8 * 2048;
   static constexpr int kTokOff = kXchOff + kXchBytes;               // gathered rows of the loaders' tile
   static constexpr int kBarOff = kTokOff + 128 * 4;
   static constexpr int kTableOff = kBarOff + 256;
@@ -154,11 +158,12 @@ struct GroupedRowsCfg {
   static constexpr int kTmemCols = 512;
 };
 
-template <bool FUSED>
-__global__ void __launch_bounds__(GroupedRowsCfg<FUSED>::kThreads, 1)
+template <bool FUSED, bool BOX = false>
+__global__ void __launch_bounds__(GroupedRowsCfg<FUSED, BOX>::kThreads, 1)
     k_grouped_rows(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                   const GroupedParams p) {
-  using Cfg = GroupedRowsCfg<FUSED>;
+                   const __grid_constant__ CUtensorMap tmO, const GroupedParams p) {
+  static_assert(!(FUSED && BOX), "the fused output is written by its threads");
+  using Cfg = GroupedRowsCfg<FUSED, BOX>;
   constexpr int S = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -444,6 +449,41 @@ __global__ void __launch_bounds__(GroupedRowsCfg<FUSED>::kThreads, 1)
               for (int j = 0; j < 32; ++j)
                 dst[j] = make_float4(lo_f(acc[2 * j]), hi_f(acc[2 * j]), lo_f(acc[2 * j + 1]), hi_f(acc[2 * j + 1]));
             }
+          } else if constexpr (BOX) {
+            // A warp's 32 rows x 128 columns leave as two boxes of 64 columns by TMA, from 8 KB of shared memory laid
+            // out as the map's 128-byte swizzle has it (a row of a box at 128 bytes, chunk c at c ^ (row % 8)). Rows
+            // of the tile that do not exist belong to the next expert: such a warp stores its rows itself, 128
+            // bytes of four rows at a time.
+            uint8_t* buf = smem + Cfg::kXchOff + warp * 8192;
+            const int rows = t.rows - q * 32;
+            bulk_wait_read_all();  // lane 0: the boxes of the previous tile
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              *reinterpret_cast<uint4*>(buf + (j >> 3) * 4096 + lane * 128 + (((j & 7) ^ (lane & 7)) * 16)) =
+                  make_uint4(pack_bf16x2(lo_f(acc[4 * j]), hi_f(acc[4 * j])),
+                             pack_bf16x2(lo_f(acc[4 * j + 1]), hi_f(acc[4 * j + 1])),
+                             pack_bf16x2(lo_f(acc[4 * j + 2]), hi_f(acc[4 * j + 2])),
+                             pack_bf16x2(lo_f(acc[4 * j + 3]), hi_f(acc[4 * j + 3])));
+            if (rows >= 32) {
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_2d(&tmO, buf, nb * 256, t.row + q * 32);
+                tma_store_2d(&tmO, buf + 4096, nb * 256 + 128, t.row + q * 32);
+                bulk_commit();
+              }
+            } else if (rows > 0) {
+              __syncwarp();
+              __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + static_cast<size_t>(t.row + q * 32) * p.ldc +
+                                   static_cast<size_t>(nb) * 128 + (lane & 7) * 8;
+#pragma unroll 4
+              for (int i = 0; i < 16; ++i) {
+                const int rr = 4 * (i >> 1) + (lane >> 3);
+                const uint4 v = *reinterpret_cast<const uint4*>(buf + (i & 1) * 4096 + rr * 128 + (((lane & 7) ^ (rr & 7)) * 16));
+                if (rr < rows) *reinterpret_cast<uint4*>(dst + static_cast<size_t>(rr) * p.ldc + (i & 1) * 64) = v;
+              }
+            }
           } else {
             // A warp's 32 rows x 32 columns at a time through 2 KB of shared memory (chunks of 16 bytes, swizzled), so
             // that a store writes whole 64-byte pieces of eight rows instead of 16 bytes of 32 rows.
@@ -504,6 +544,7 @@ __global__ void __launch_bounds__(GroupedRowsCfg<FUSED>::kThreads, 1)
         named_bar_sync(1, 256);  // amax_x is free for the next tile
       }
     }
+    if constexpr (BOX) bulk_wait_read_all();  // the last boxes have left shared memory
   }
   tc_fence_before();
   __syncthreads();

@@ -90,6 +90,16 @@ int launch_grouped_tokens(const CUtensorMap& tmW, const CUtensorMap& tmX, const 
                             "k_grouped_tokens launch", tmW, tmX, p, log_s);
 }
 
+template <bool FUSED, bool BOX>
+int launch_grouped_rows(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmO, const bs::GroupedParams& p,
+                        int num_sms, cudaStream_t s) {
+  using Cfg = bs::GroupedRowsCfg<FUSED, BOX>;
+  constexpr auto kern = bs::k_grouped_rows<FUSED, BOX>;
+  const int rc = prepare_kernel<kern>(Cfg::kSmemBytes, Cfg::Regs::kLaunch);
+  if (rc != BS_OK) return rc;
+  return launch_pdl(kern, num_sms, Cfg::kThreads, Cfg::kSmemBytes, s, "k_grouped_rows launch", tmA, tmB, tmO, p);
+}
+
 template <bool FUSED>
 int run_grouped(const void* A, const void* B, const bs::GroupedParams& p, int rows_hint, cudaStream_t s, int num_sms) {
   const int K = p.KB * 128;
@@ -103,11 +113,16 @@ int run_grouped(const void* A, const void* B, const bs::GroupedParams& p, int ro
     case 32: return launch_grouped_tokens<FUSED, 32>(tmB, tmA, p, g.log_s, num_sms, s);
     default: break;
   }
-  using Cfg = bs::GroupedRowsCfg<FUSED>;
-  constexpr auto kern = bs::k_grouped_rows<FUSED>;
-  const int rc = prepare_kernel<kern>(Cfg::kSmemBytes, Cfg::Regs::kLaunch);
-  if (rc != BS_OK) return rc;
-  return launch_pdl(kern, num_sms, Cfg::kThreads, Cfg::kSmemBytes, s, "k_grouped_rows launch", tmA, tmB, p);
+  if constexpr (!FUSED) {
+    // measured at the kernel: boxes pay from about 128 rows per expert on
+    if (!p.out_f32 && rows_hint > 128ll * p.E) {
+      CUtensorMap tmO;
+      if (make_map(&tmO, p.out, static_cast<uint64_t>(p.nblk) * 256, p.R, static_cast<uint64_t>(p.ldc) * 2, 128, 32) != BS_OK)
+        return BS_ERR_TMAP;
+      return launch_grouped_rows<false, true>(tmA, tmB, tmO, p, num_sms, s);
+    }
+  }
+  return launch_grouped_rows<FUSED, false>(tmA, tmB, tmA, p, num_sms, s);
 }
 
 int validate_grouped(const void* A, const void* B, const void* out, const float* As, const float* Bs, const float* qs,
