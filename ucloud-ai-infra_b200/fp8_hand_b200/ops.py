@@ -262,10 +262,14 @@ def _one_device(*ts: torch.Tensor) -> int:
     """Index of the CUDA device that holds every tensor."""
     index = ts[0].get_device()
     for t in ts:
-        if t.get_device() != index or index < 0 or not t.is_cuda:
+        if t.get_device() != index or index < 0:
             _cuda(*ts)
             raise ValueError("all tensors must be on the same CUDA device")
     return index
+
+
+def _matrix(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)  # a third cheaper than torch.empty
 
 
 def _local_experts(experts, num_experts: int) -> tuple[int, int]:
@@ -285,7 +289,7 @@ def _offsets_and_scratch(lib, T: int, count: int, device: torch.device):
     """offsets [count + 1], and the address and bytes of the scratch behind it (one allocation)."""
     scratch = lib.bs_fp8_moe_scratch_bytes(T, count)
     if not scratch:
-        return torch.empty(count + 1, dtype=torch.int32, device=device), None, 0
+        return torch.empty_strided((count + 1,), (1,), dtype=torch.int32, device=device), None, 0
     buf = torch.empty(count + 1 + scratch // 4, dtype=torch.int32, device=device)
     return buf[:count + 1], buf.data_ptr() + 4 * (count + 1), scratch
 
@@ -311,13 +315,14 @@ def moe_route(logits: torch.Tensor, top_k: int, *, renormalize: bool = True, sca
             logits = logits.contiguous()
         ld = E
     lib, dev = _native.lib(), logits.device
-    weights, ids, row_token, slot_row = torch.empty((4, T, top_k), dtype=torch.int32, device=dev).unbind()
+    weights = _matrix(T, top_k, torch.float32, dev)
+    ids, slot_row = torch.empty((2, T, top_k), dtype=torch.int32, device=dev).unbind()
+    row_token = torch.empty_strided((T * top_k,), (1,), dtype=torch.int32, device=dev)
     offsets, scratch, scratch_bytes = _offsets_and_scratch(lib, T, count, dev)
-    base, step = weights.data_ptr(), 4 * T * top_k
     _native.call(lib.bs_fp8_moe_route, "bs_fp8_moe_route", index, logits.data_ptr(), f32, ld, T, E, top_k, renormalize,
-                 scale, begin, count, base, base + step, offsets.data_ptr(), base + 2 * step, base + 3 * step, scratch,
-                 scratch_bytes)
-    return MoeRoute(weights.view(torch.float32), ids, offsets, row_token.view(-1), slot_row, E)
+                 scale, begin, count, weights.data_ptr(), ids.data_ptr(), offsets.data_ptr(), row_token.data_ptr(),
+                 slot_row.data_ptr(), scratch, scratch_bytes)
+    return MoeRoute(weights, ids, offsets, row_token, slot_row, E)
 
 
 def moe_dispatch(ids: torch.Tensor, weights: torch.Tensor | None, num_experts: int, *,
@@ -394,8 +399,7 @@ def grouped_gemm(A: torch.Tensor, B: torch.Tensor, As: torch.Tensor, Bs: torch.T
     if not gather and rows_a < R:
         raise ValueError(f"A has {rows_a} rows, the route has {R}")
     if out is None:
-        out = torch.empty((R, N), dtype=out_dtype, device=A.device)
-        ldc = N
+        out, ldc = _matrix(R, N, out_dtype, A.device), N
     else:
         if out.shape != (R, N) or out.get_device() != index or out.stride(1) != 1:
             raise ValueError("output must be [T * k, N] with contiguous rows, on the same device")
@@ -418,8 +422,8 @@ def grouped_gemm_silu_quant(A: torch.Tensor, B: torch.Tensor, As: torch.Tensor, 
     if N2 % (2 * BLOCK):
         raise ValueError("gate_up rows must be a multiple of 256")
     dev = A.device
-    Q = torch.empty((R, N2 // 2), dtype=E4M3, device=dev)
-    Qs = torch.empty((R, N2 // (2 * BLOCK)), dtype=torch.float32, device=dev)
+    Q = _matrix(R, N2 // 2, E4M3, dev)
+    Qs = _matrix(R, N2 // (2 * BLOCK), torch.float32, dev)
     _native.call(_native.lib().bs_fp8_grouped_gemm_silu_quant, "bs_fp8_grouped_gemm_silu_quant", index, A.data_ptr(),
                  B.data_ptr(), Q.data_ptr(), As.data_ptr(), Bs.data_ptr(), Qs.data_ptr(), route.offsets.data_ptr(),
                  route.row_token.data_ptr(), rows_a, R, hint, E, N2, K, b_tiled)
@@ -429,20 +433,44 @@ def grouped_gemm_silu_quant(A: torch.Tensor, B: torch.Tensor, As: torch.Tensor, 
 def _rows16(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     """(t with contiguous rows that start on 16 bytes, copied where they do not; its row stride)."""
     rows, n = t.shape
-    ld, inner = t.stride()
-    if rows <= 1:
+    if t.is_contiguous():
         ld = n
-    if inner != 1 or ld < n or (ld * t.element_size()) % 16 or t.data_ptr() % 16:
+    else:
+        ld, inner = t.stride()
+        if rows <= 1:
+            ld = n
+        if inner != 1 or ld < n:
+            return t.clone(memory_format=torch.contiguous_format), n
+    if (ld * t.element_size()) % 16 or t.data_ptr() % 16:
         return t.clone(memory_format=torch.contiguous_format), n
     return t, ld
 
 
-def _norm_weight(w: torch.Tensor | None, H: int, index: int) -> int | None:
-    if w is None:
-        return None
-    if w.dtype != torch.bfloat16 or w.shape != (H,) or w.get_device() != index or w.stride(0) != 1 or w.data_ptr() % 16:
+def _norm_weight(w: torch.Tensor, H: int, index: int) -> int:
+    """The address of a norm's weight."""
+    at = w.data_ptr()
+    if w.dtype != torch.bfloat16 or w.shape != (H,) or w.get_device() != index or at % 16 or not w.is_contiguous():
         raise ValueError("norm weights must be contiguous, 16-byte aligned bf16 [H] on the same device")
-    return w.data_ptr()
+    return at
+
+
+def _gate(gate: torch.Tensor, T: int, H: int, index: int) -> tuple[torch.Tensor, int, int]:
+    """(the gate, copied where its rows are not contiguous; its kind in the C-ABI; its row stride)."""
+    if gate.dtype != torch.bfloat16 or gate.get_device() != index:
+        raise ValueError("gate must be bf16 on the same device")
+    if gate.dim() == 1 and gate.shape[0] == H:
+        if gate.data_ptr() % 16 or not gate.is_contiguous():
+            gate = gate.clone(memory_format=torch.contiguous_format)
+        return gate, 1, 0
+    if gate.dim() != 2 or gate.shape[0] != T or gate.shape[1] not in (1, H):
+        raise ValueError("gate must be [H], [T, 1] or [T, H]")
+    if gate.shape[1] == 1:
+        ld = gate.stride(0) if T > 1 else 1
+        if ld < 1:
+            gate, ld = gate.contiguous(), 1
+        return gate, 2, ld
+    gate, ld = _rows16(gate)
+    return gate, 3, ld
 
 
 def block_norm_quant(y: torch.Tensor, residual: torch.Tensor | None, *, post_weight: torch.Tensor | None = None,
@@ -462,23 +490,27 @@ def block_norm_quant(y: torch.Tensor, residual: torch.Tensor | None, *, post_wei
     if y.dim() != 2 or y.dtype != bf16:
         raise ValueError("y must be bf16 [rows, H]")
     rows_y, hy = y.shape
+    index, dev = y.get_device(), y.device
     if residual is None:
-        wide, index, H = False, _one_device(y), hy
+        wide, H = False, hy
         T = rows_y if route is None else route.slot_row.shape[0]
     else:
         wide = residual.dtype == torch.float32
         if residual.dim() != 2 or not (wide or residual.dtype == bf16):
             raise ValueError("residual must be bf16 or fp32 [T, H]")
-        index = _one_device(y, residual)
+        if index < 0 or residual.get_device() != index:
+            _one_device(y, residual)
         T, H = residual.shape
-    dev, h_type = y.device, torch.float32 if wide else bf16
+    if index < 0:
+        _one_device(y)
     if H % BLOCK or not 0 < H <= 16384:
         raise ValueError("H must be a multiple of 128, at most 16384")
     if hy != H or (route is None and rows_y != T):
         raise ValueError("y must have residual's shape (or be a route's rows)")
+    h_type = torch.float32 if wide else bf16
     given = out
     if out is None:
-        out, ldo = torch.empty((T, H), dtype=h_type, device=dev), H
+        out, ldo = _matrix(T, H, h_type, dev), H
     else:
         if out.shape != (T, H) or out.dtype != h_type or out.get_device() != index:
             raise ValueError("out must be like residual")
@@ -490,24 +522,10 @@ def block_norm_quant(y: torch.Tensor, residual: torch.Tensor | None, *, post_wei
     if residual is not None:
         residual, ldr = (out, ldo) if residual is given else _rows16(residual)
         r_ptr = residual.data_ptr()
-    post, pre = _norm_weight(post_weight, H, index), _norm_weight(pre_weight, H, index)
+    post = None if post_weight is None else _norm_weight(post_weight, H, index)
     kind, ldg, g_ptr = 0, 0, None
     if gate is not None:
-        if gate.dtype != bf16 or gate.get_device() != index:
-            raise ValueError("gate must be bf16 on the same device")
-        if gate.dim() == 1:
-            _need(gate.shape[0] == H, "gate must be [H], [T, 1] or [T, H]")
-            if gate.stride(0) != 1 or gate.data_ptr() % 16:
-                gate = gate.clone(memory_format=torch.contiguous_format)
-            kind = 1
-        else:
-            _need(gate.dim() == 2 and gate.shape[0] == T and gate.shape[1] in (1, H), "gate must be [H], [T, 1] or [T, H]")
-            if gate.shape[1] == 1:
-                if T > 1 and gate.stride(0) < 1:
-                    gate = gate.contiguous()
-                kind, ldg = 2, gate.stride(0) if T > 1 else 1
-            else:
-                kind, (gate, ldg) = 3, _rows16(gate)
+        gate, kind, ldg = _gate(gate, T, H, index)
         g_ptr = gate.data_ptr()
     w_ptr = s_ptr = None
     k = 0
@@ -515,23 +533,23 @@ def block_norm_quant(y: torch.Tensor, residual: torch.Tensor | None, *, post_wei
         w, rows = route.weights, route.slot_row
         if w is None or w.shape != rows.shape or rows.shape[0] != T:
             raise ValueError("the route must have weights, and a token for each row of the residual")
-        _one_device(y, w, rows)
+        if w.get_device() != index or rows.get_device() != index:
+            _one_device(y, w, rows)
         if w.dtype != torch.float32 or rows.dtype != torch.int32 or not (w.is_contiguous() and rows.is_contiguous()):
             raise ValueError("the route's weights and rows must be contiguous fp32 and int32")
         w_ptr, s_ptr, k = w.data_ptr(), rows.data_ptr(), rows.shape[1]
-    A = As = V = a_ptr = as_ptr = v_ptr = None
-    if pre is not None:
-        A = torch.empty((T, H), dtype=E4M3, device=dev)
-        As = torch.empty((T, H // BLOCK), dtype=torch.float32, device=dev)
-        a_ptr, as_ptr = A.data_ptr(), As.data_ptr()
+    if pre_weight is None:
         if norm_out:
-            V = torch.empty((T, H), dtype=bf16, device=dev)
-            v_ptr = V.data_ptr()
-    elif norm_out:
-        raise ValueError("norm_out needs pre_weight")
+            raise ValueError("norm_out needs pre_weight")
+        A = As = V = pre = a_ptr = as_ptr = v_ptr = None
+    else:
+        pre = _norm_weight(pre_weight, H, index)
+        A, As = _matrix(T, H, E4M3, dev), _matrix(T, H // BLOCK, torch.float32, dev)
+        V = _matrix(T, H, bf16, dev) if norm_out else None
+        a_ptr, as_ptr, v_ptr = A.data_ptr(), As.data_ptr(), _native.ptr(V)
     _native.call(_native.lib().bs_fp8_block_norm_quant, "bs_fp8_block_norm_quant", index, y.data_ptr(), ldy, rows_y, w_ptr,
-                 s_ptr, k, r_ptr, ldr, out.data_ptr(), ldo, wide, post, g_ptr, kind, ldg, scale,
-                 residual_scale, pre, eps, a_ptr, as_ptr, v_ptr, T, H)
-    if pre is None:
+                 s_ptr, k, r_ptr, ldr, out.data_ptr(), ldo, wide, post, g_ptr, kind, ldg, scale, residual_scale, pre, eps,
+                 a_ptr, as_ptr, v_ptr, T, H)
+    if pre_weight is None:
         return out
     return (out, A, As, V) if norm_out else (out, A, As)
