@@ -55,16 +55,23 @@ struct BlockParams {
 constexpr int kBlockMaxStages = 16;
 constexpr int kBlockRingBytes = 100 * 1024;  // two CTAs per SM
 
-// Rows per stage (a power of two, at least two stages fit) and stages.
-__host__ __device__ inline int block_stage_rows(int k, int H) {
-  int g = k >= 3 ? 4 : k;
-  while (g > 1 && 2 * g * 2 * H > kBlockRingBytes) g >>= 1;
-  return g;
+constexpr int kBlockResSlots = 2;
+
+// The ring of a launch: two residual rows, and stages of G rows (a power of two), two at least.
+struct BlockRing {
+  int G, stages, res_bytes;  // res_bytes: a residual row's, 0 without one
+  __host__ __device__ int bytes(int H) const { return kBlockResSlots * res_bytes + stages * G * 2 * H; }
+};
+__host__ __device__ inline BlockRing block_ring(int k, int H, int res_bytes) {
+  BlockRing r = {k >= 3 ? 4 : k, 0, res_bytes};
+  const int room = kBlockRingBytes - kBlockResSlots * res_bytes;
+  while (r.G > 1 && 2 * r.G * 2 * H > room) r.G >>= 1;
+  const int n = room / (r.G * 2 * H);
+  r.stages = n < 2 ? 2 : n > kBlockMaxStages ? kBlockMaxStages : n;
+  return r;
 }
-__host__ __device__ inline int block_stages(int rows, int H) {
-  const int n = kBlockRingBytes / (rows * 2 * H);
-  return n > kBlockMaxStages ? kBlockMaxStages : n;
-}
+// The widest: fp32 residual rows and one-row stages of kBlockMaxH elements.
+constexpr int kBlockMaxSmem = kBlockResSlots * 4 * kBlockMaxH + 2 * 2 * kBlockMaxH;
 
 // Sum over the `threads` consumer threads in a fixed order: a butterfly per warp, then one over the (at most 16) warp totals.
 // `buf` is not reused before the next barrier.
@@ -98,20 +105,27 @@ __device__ __forceinline__ float amax_div_448(float amax) {
 
 template <int C, bool WIDE>
 __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block_norm(const BlockParams p) {
-  extern __shared__ __align__(128) uint8_t ring[];  // [stages][G rows][2 H]
+  extern __shared__ __align__(128) uint8_t block_smem[];  // residual rows, then [stages][G rows][2 H]
   __shared__ float sums[2][2][kBlockMaxThreads / 32];  // by row parity and norm
   __shared__ uint64_t full[kBlockMaxStages], empty[kBlockMaxStages];
+  __shared__ uint64_t rfull[kBlockResSlots], rempty[kBlockResSlots];
   __shared__ float4 weight[kBlockMaxStages];
   __shared__ int there[kBlockMaxStages];  // bit g: row g of the stage is one (its slot has a row)
   __shared__ volatile int abort_flag;
   const int t = threadIdx.x, nt = static_cast<int>(blockDim.x) - 32, lane = t & 31;
   const int nch = p.H / 8, row_bytes = 2 * p.H;
   const int k = p.weights ? p.k : 1;
-  const int G = block_stage_rows(k, p.H), stages = block_stages(G, p.H);
+  const BlockRing br = block_ring(k, p.H, p.residual ? (WIDE ? 4 : 2) * p.H : 0);
+  const int G = br.G, stages = br.stages, res_bytes = br.res_bytes;
+  uint8_t* ring = block_smem + kBlockResSlots * res_bytes;
   if (t == 0) {
     for (int i = 0; i < stages; ++i) {
       mbar_init(&full[i], 2);  // both by the producer: the bytes to come, and the weights
       mbar_init(&empty[i], nt / 32);
+    }
+    for (int i = 0; i < kBlockResSlots; ++i) {
+      mbar_init(&rfull[i], 1);
+      mbar_init(&rempty[i], nt / 32);
     }
     abort_flag = 0;
     fence_mbar_init();
@@ -123,8 +137,8 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
   if (t >= nt) {
     // ------------------------------------------------------------ producer
     const uint64_t policy = policy_evict_first();
-    int st = 0;
-    uint32_t ph = 0;
+    int st = 0, rs = 0;
+    uint32_t ph = 0, rph = 0;
     bool ok = true;
     // lane s holds slot s of the next token
     auto slot = [&](int row, int& r, float& w) {
@@ -145,6 +159,23 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
       const int my_r = next_r;
       const float my_w = next_w;
       slot(row + gridDim.x, next_r, next_w);
+      if (res_bytes) {
+        if (lane == 0) {
+          ok = mbar_wait(&rempty[rs], rph ^ 1, &abort_flag, p.status, kErrTimeoutEmpty);
+          if (ok) {
+            mbar_arrive_expect_tx(&rfull[rs], res_bytes);
+            bulk_load(block_smem + rs * res_bytes,
+                      static_cast<const uint8_t*>(p.residual) + static_cast<long long>(row) * p.ldr * (WIDE ? 4 : 2), res_bytes,
+                      &rfull[rs], policy);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        if (++rs == kBlockResSlots) {
+          rs = 0;
+          rph ^= 1;
+        }
+      }
       const uint32_t has = __ballot_sync(0xffffffffu, static_cast<unsigned>(my_r) < static_cast<unsigned>(p.rows_y));
       for (int s = 0; s < k; s += G) {
         if (lane == 0) ok = mbar_wait(&empty[st], ph ^ 1, &abort_flag, p.status, kErrTimeoutEmpty);
@@ -193,28 +224,16 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
       gch[j] = chunk(channel, t + nt * j);
     }
   }
-  int st = 0;
-  uint32_t ph = 0;
+  int st = 0, rs = 0;
+  uint32_t ph = 0, rph = 0;
   bool ok = true;
   for (int row = blockIdx.x, parity = 0; row < p.T; row += gridDim.x, parity ^= 1) {
     // in flight while the rows are added up
-    uint4 res[C][WIDE ? 2 : 1], gv[kKeep ? C : 1];
+    uint4 gv[kKeep ? C : 1];
     float gt = p.scale;
+    if constexpr (kKeep) {
 #pragma unroll
-    for (int j = 0; j < C; ++j) {
-      const int c = t + nt * j;
-      if (c < nch) {
-        if (!p.residual) {
-          res[j][0] = res[j][WIDE ? 1 : 0] = make_uint4(0, 0, 0, 0);
-        } else if constexpr (WIDE) {
-          const uint4* rr = reinterpret_cast<const uint4*>(static_cast<const float*>(p.residual) + row * p.ldr + c * 8);
-          res[j][0] = rr[0];
-          res[j][1] = rr[1];
-        } else {
-          res[j][0] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.residual) + row * p.ldr + c * 8);
-        }
-        if constexpr (kKeep) gv[j] = p.gate_kind == kGateFull ? chunk(p.gate + row * p.ldg, c) : gch[j];
-      }
+      for (int j = 0; j < C; ++j) gv[j] = p.gate_kind == kGateFull ? chunk(p.gate + row * p.ldg, t + nt * j) : gch[j];
     }
     if (p.gate_kind == kGateToken) gt = __bfloat162float(__ldg(p.gate + row * p.ldg)) * p.scale;
 
@@ -276,6 +295,8 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
         for (int e = 0; e < 4; ++e) z[j][e] = fmul2(fmul2(z[j][e], rs2), bf16x2_to_f2(w[e]));
       }
     }
+    if (res_bytes && ok) ok = mbar_wait_warp(&rfull[rs], rph, &abort_flag, p.status, kErrTimeoutFull);
+    const uint4* res = reinterpret_cast<const uint4*>(block_smem + rs * res_bytes);
     const uint64_t gs2 = pack_f2(gt, gt), a2 = pack_f2(p.residual_scale, p.residual_scale);
 #pragma unroll
     for (int j = 0; j < C; ++j) {
@@ -285,14 +306,17 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
         if constexpr (kKeep) g4 = gv[j];
         else g4 = chunk(p.gate_kind == kGateFull ? p.gate + row * p.ldg : channel, c);
         const uint32_t* gw = reinterpret_cast<const uint32_t*>(&g4);
-        const uint32_t* rw = reinterpret_cast<const uint32_t*>(&res[j][0]);
+        uint4 rv[WIDE ? 2 : 1];
+#pragma unroll
+        for (int i = 0; i < (WIDE ? 2 : 1); ++i) rv[i] = res_bytes && ok ? res[WIDE ? 2 * c + i : c] : make_uint4(0, 0, 0, 0);
+        const uint32_t* rw = reinterpret_cast<const uint32_t*>(&rv[0]);
         const bool per_element = p.gate_kind == kGateChannel || p.gate_kind == kGateFull;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint64_t g = per_element ? fmul2(bf16x2_to_f2(gw[e]), gs2) : gs2;
           uint64_t r;
           if constexpr (WIDE) {
-            const uint32_t* ww = reinterpret_cast<const uint32_t*>(&res[j][e >> 1]);
+            const uint32_t* ww = reinterpret_cast<const uint32_t*>(&rv[e >> 1]);
             r = static_cast<uint64_t>(ww[(2 * e) & 3]) | (static_cast<uint64_t>(ww[(2 * e + 1) & 3]) << 32);
           } else {
             r = bf16x2_to_f2(rw[e]);
@@ -310,6 +334,14 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
                            pack_bf16x2(lo_f(z[j][2]), hi_f(z[j][2])), pack_bf16x2(lo_f(z[j][3]), hi_f(z[j][3])));
           }
         }
+      }
+    }
+    if (res_bytes) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&rempty[rs]);
+      if (++rs == kBlockResSlots) {
+        rs = 0;
+        rph ^= 1;
       }
     }
     if (p.pre) {

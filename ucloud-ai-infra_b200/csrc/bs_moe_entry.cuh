@@ -26,7 +26,7 @@ int launch_route(const bs::RouteParams& p, int f32, int grid, cudaStream_t s) {
 int run_route(bs::RouteParams& p, int f32, void* scratch, size_t scratch_bytes, void* stream) {
   if (p.T < 0 || p.k <= 0 || p.k > bs::kMaxTopK || p.E <= 0 || p.E > bs::kMaxExperts) return BS_ERR_ARG;
   if (p.e_begin < 0 || p.e_count <= 0 || p.e_count > p.E - p.e_begin) return BS_ERR_ARG;
-  if (static_cast<long long>(p.T) * p.k >= (1ll << 31)) return BS_ERR_ARG;
+  if (static_cast<long long>(p.T) * p.k > (1ll << 30)) return BS_ERR_ARG;  // 32-bit rows, with room for a CTA's tokens
   if (!p.offsets || (p.T > 0 && (!p.row_token || !p.slot_row))) return BS_ERR_ARG;
   DeviceState* d = device_state();
   if (!d) return BS_ERR_CUDA;
@@ -133,7 +133,8 @@ int validate_grouped(const void* A, const void* B, const void* out, const float*
   if (rc != BS_OK || R == 0) return rc;
   if (!offsets || rows_a == 0 || (!row_token && rows_a < R)) return BS_ERR_ARG;
   // 32-bit tile counts and TMA coordinates
-  if (static_cast<long long>(E) * N * (b_tiled ? K / 128 : 1) >= (1ll << 31)) return BS_ERR_ARG;
+  // (one weight block past the last expert's is addressed, and read as zeros, where N / 128 is odd)
+  if ((static_cast<long long>(E) * N + 128) * (b_tiled ? K / 128 : 1) >= (1ll << 31)) return BS_ERR_ARG;
   if (static_cast<long long>(rows_a) * (K / 16) >= (1ll << 32)) return BS_ERR_ARG;
   if ((static_cast<long long>(R) / 16 + E) * (N / 128) >= (1ll << 31)) return BS_ERR_ARG;
   return BS_OK;
@@ -160,10 +161,9 @@ bs::GroupedParams grouped_params(const void* A, const float* As, const float* Bs
 template <int C, bool WIDE>
 int launch_block(const bs::BlockParams& p, int threads, int num_sms, cudaStream_t s) {
   constexpr auto kern = bs::k_block_norm<C, WIDE>;
-  const int rc = prepare_kernel<kern>(bs::kBlockRingBytes, 0);
+  const int rc = prepare_kernel<kern>(bs::kBlockMaxSmem, 0);
   if (rc != BS_OK) return rc;
-  const int rows = bs::block_stage_rows(p.weights ? p.k : 1, p.H);
-  const int smem = bs::block_stages(rows, p.H) * rows * 2 * p.H;
+  const int smem = bs::block_ring(p.weights ? p.k : 1, p.H, p.residual ? (WIDE ? 4 : 2) * p.H : 0).bytes(p.H);
   int per_sm = 0;
   if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads + 32, smem) != cudaSuccess || per_sm < 1)
     per_sm = 1;
