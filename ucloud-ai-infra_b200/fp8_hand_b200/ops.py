@@ -1,5 +1,6 @@
 """Tensor-level entry points over the C-ABI: activation quant, weight pre-pack, block-scaled FP8
-GEMM and the fused gate_up + SiLU*up + quant front half.
+GEMM and the fused gate_up + SiLU*up + quant front half; for mixtures of experts the router with its
+dispatch plan, the products grouped by expert, and the block's end with its norms.
 
 All functions take CUDA tensors, launch on the current stream of the tensors' device, never
 synchronise and never fall back: a tensor outside the contract raises ValueError, a library
