@@ -696,12 +696,13 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
     tmem_alloc(tmem_slot, Cfg::kTmemCols);
     tmem_relinquish();
   }
-  grid_dep_wait();
-  if (warp == 0) build_table(table, p, NT, num_n);
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // every CTA's barriers exist before a remote arrival
   tc_fence_after();
+  grid_dep_wait();  // what follows may read the previous kernel's output
+  if (warp == 0) build_table(table, p, NT, num_n);
+  __syncthreads();
   const uint32_t tmem = *tmem_slot;
   const int num_tiles = table.tiles;
   const int first = static_cast<int>(blockIdx.x) >> log_s, step = static_cast<int>(gridDim.x) >> log_s;
