@@ -1,7 +1,7 @@
 // Block-scaled FP8 products grouped by expert, ragged row counts, for sm_100a:
 //     C[r, n] = sum_kb P_kb[r, n] * (As[src(r), kb] * Bs[e, n / 128, kb]),  offsets[e] <= r < offsets[e + 1]
 // P_kb the fp32 product of one 128-wide K block of e4m3 rows and expert e's e4m3 weights, promoted as in
-// bs_prefill.cuh. src(r) = row_token[r] (the rows are read in place, by a gathering TMA load) or r. FUSED: the
+// bs_prefill.cuh. src(r) = row_token[r] (the rows are read in place, no copy in row order is made) or r. FUSED: the
 // weights are [gate; up], and the output is Q, Qs of silu(g) * u per 128-column group (bs_prefill.cuh).
 //
 // The row counts are known on the device only: every CTA turns the offsets into a table of the experts that have
@@ -9,9 +9,14 @@
 // of one expert are adjacent, row tiles fastest, so an expert's weights come from HBM once and its row tiles
 // share them in L2.
 //
-// Two kernels. k_grouped_rows: 128 rows x 256 weight columns per tile, rows on the MMA's 128 lanes: tensor bound,
-// for experts with many rows. k_grouped_tokens: 128 weight rows on the lanes, up to NT rows on the columns: bound by
-// the weights' stream, for experts with few rows.
+// Two kernels (the choice between them, with both measured: grouped_plan in bs_moe_entry.cuh).
+//   k_grouped_rows    128 rows x 256 weight columns per tile, rows on the MMA's 128 lanes, for experts with many rows. Bound
+//                     by the promotion of each K block's partial and by power: 8192 tokens x 8 of 64 experts, fused
+//                     5120 -> 2 x 1024 880 us, plain 1024 -> 5120 483 us (1.5 PFLOP/s, at 1.45-1.65 GHz under the
+//                     1000 W limit; a tile costs 128 rows whatever it holds)
+//   k_grouped_tokens  128 weight rows on the lanes, up to 16 or 32 rows on the columns, for experts with few rows. Bound by
+//                     the weights' stream: 61 tokens x 8 of 64 experts, the same products: 101 us (6.65 TB/s), 58 us;
+//                     one token: 18.5 us for 84 MB, of which some 6 us are the start (the plan, the first boxes) and end
 #pragma once
 #include "bs_common.cuh"
 #include "bs_prefill.cuh"
@@ -135,9 +140,10 @@ __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wai
 // ---------------------------------------------------------------- many rows per expert
 // Roles, stages, TMEM buffers and the promotion are those of k_prefill (bs_prefill.cuh). When the rows are gathered,
 // warps 10 and 11 bring them, 64 rows each, with 16-byte cp.async copies written where the 128-byte swizzle of a TMA
-// load would put them (chunk c of row r at chunk c ^ (r % 8)). A gathering TMA load (four rows each) was measured first
-// and is the bound of the kernel there: 8192 tokens x 8 of 64 experts, K = 5120, N = 2048, one product: 1894 us gathered
-// by TMA, 843 us with the rows already in order.
+// load would put them (chunk c of row r at chunk c ^ (r % 8)). 8192 tokens x 8 of 64 experts, K = 5120, N = 2048, plain:
+// 1894 us with gathering TMA loads (four rows each, one every 50 ns), 819 us with the loaders, 790 us with the rows
+// already in order. The loaders share the promotion warps' issue slots, so their instructions per copy count: 971 us with
+// 64-bit row products and a shared-memory load for each copy.
 // BOX (plain bf16 output): whole 32-row pieces of a tile leave by TMA from 64 KB of shared memory, at three stages. Measured
 // (64 experts, K = 1024, N = 5120; without and with): mean 30 rows per expert 68 and 75 us, 125 rows 102 and 102, 1024
 // rows 516 and 493.
