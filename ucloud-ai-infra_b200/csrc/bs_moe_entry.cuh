@@ -164,11 +164,14 @@ int launch_block(const bs::BlockParams& p, int threads, int num_sms, cudaStream_
   const int rc = prepare_kernel<kern>(bs::kBlockMaxSmem, 0);
   if (rc != BS_OK) return rc;
   const int smem = bs::block_ring(p.weights ? p.k : 1, p.H, p.residual ? (WIDE ? 4 : 2) * p.H : 0).bytes(p.H);
-  int per_sm = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads + 32, smem) != cudaSuccess || per_sm < 1)
-    per_sm = 1;
-  cudaGetLastError();
-  const int grid = p.T < per_sm * num_sms ? p.T : per_sm * num_sms;
+  int grid = p.T;  // a CTA per token, or as many as fit
+  if (p.T > num_sms) {
+    int per_sm = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads + 32, smem) != cudaSuccess || per_sm < 1)
+      per_sm = 1;
+    cudaGetLastError();
+    grid = std::min(p.T, per_sm * num_sms);
+  }
   return launch_pdl(kern, grid, threads + 32, smem, s, "k_block_norm launch", p);
 }
 

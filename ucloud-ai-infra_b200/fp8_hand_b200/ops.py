@@ -317,7 +317,7 @@ def moe_route(logits: torch.Tensor, top_k: int, *, renormalize: bool = True, sca
         ld = E
     lib, dev = _native.lib(), logits.device
     weights = _matrix(T, top_k, torch.float32, dev)
-    ids, slot_row = torch.empty((2, T, top_k), dtype=torch.int32, device=dev).unbind()
+    ids, slot_row = _matrix(T, top_k, torch.int32, dev), _matrix(T, top_k, torch.int32, dev)
     row_token = torch.empty_strided((T * top_k,), (1,), dtype=torch.int32, device=dev)
     offsets, scratch, scratch_bytes = _offsets_and_scratch(lib, T, count, dev)
     _native.call(lib.bs_fp8_moe_route, "bs_fp8_moe_route", index, logits.data_ptr(), f32, ld, T, E, top_k, renormalize,
