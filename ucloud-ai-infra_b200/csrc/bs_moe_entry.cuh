@@ -4,23 +4,61 @@
 
 namespace {
 
-// Tokens per CTA of the route kernels: one round of a CTA's warps, more when that would take more CTAs than fit on the
+// CTAs that a cluster of the route kernel may have on the current device: 16 where such a cluster can run, else the
+// portable 8.
+template <int VPL>
+int route_cluster() {
+  struct State {
+    std::once_flag once[kMaxDevices];
+    int n[kMaxDevices];
+  };
+  static State st;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 8;
+  std::call_once(st.once[dev], [&] {
+    st.n[dev] = 8;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(16);
+    cfg.blockDim = dim3(bs::kRouteThreads);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 16;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaFuncSetAttribute(bs::k_moe_route<VPL>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+        cudaOccupancyMaxActiveClusters(&n, bs::k_moe_route<VPL>, &cfg) == cudaSuccess && n > 0)
+      st.n[dev] = 16;
+    cudaGetLastError();
+  });
+  return st.n[dev];
+}
+
+// Tokens per CTA of the two-launch form: one round of a CTA's warps, more when that would take more CTAs than fit on the
 // device at once, two per SM (k_moe_place reads every CTA's counts).
 int route_tokens_per_cta(int T, int num_sms) {
-  const int at_once = bs::kRouteFuse * 2 * num_sms;
-  const int rounds = T / at_once + (T % at_once != 0);
-  return bs::kRouteFuse * (rounds > 1 ? rounds : 1);
+  const int at_once = bs::kRouteRound * 2 * num_sms;
+  return bs::kRouteRound * (T / at_once + (T % at_once != 0));
 }
 int route_grid(int T, int num_sms) {
   const int per = route_tokens_per_cta(T, num_sms);
-  return T > 0 ? (T + per - 1) / per : 1;
+  return (T + per - 1) / per;
 }
 
 template <int VPL>
-int launch_route(const bs::RouteParams& p, int f32, int grid, cudaStream_t s) {
-  int rc = launch_pdl(bs::k_moe_route<VPL>, grid, bs::kRouteThreads, 0, s, "k_moe_route launch", p, f32);
-  if (rc == BS_OK && grid > 1) rc = launch_pdl(bs::k_moe_place, grid, bs::kRouteThreads, 0, s, "k_moe_place launch", p);
-  return rc;
+int launch_route(bs::RouteParams& p, int f32, int num_sms, cudaStream_t s) {
+  if (!p.hist) {
+    const int rounds = p.T <= bs::kRouteRound * route_cluster<VPL>() ? 1 : 2;  // kRouteCluster: two rounds of eight CTAs
+    p.per_cta = bs::kRouteRound * rounds;
+    const int grid = p.T > 0 ? (p.T + p.per_cta - 1) / p.per_cta : 1;
+    return launch_pdl_cluster(bs::k_moe_route<VPL>, grid, bs::kRouteThreads, 0, grid, s, "k_moe_route launch", p, f32);
+  }
+  p.per_cta = route_tokens_per_cta(p.T, num_sms);
+  const int grid = route_grid(p.T, num_sms);
+  const int rc = launch_pdl(bs::k_moe_route<VPL>, grid, bs::kRouteThreads, 0, s, "k_moe_route launch", p, f32);
+  return rc != BS_OK ? rc : launch_pdl(bs::k_moe_place, grid, bs::kRouteThreads, 0, s, "k_moe_place launch", p);
 }
 
 int run_route(bs::RouteParams& p, int f32, void* scratch, size_t scratch_bytes, void* stream) {
@@ -30,20 +68,19 @@ int run_route(bs::RouteParams& p, int f32, void* scratch, size_t scratch_bytes, 
   if (!p.offsets || (p.T > 0 && (!p.row_token || !p.slot_row))) return BS_ERR_ARG;
   DeviceState* d = device_state();
   if (!d) return BS_ERR_CUDA;
-  p.per_cta = route_tokens_per_cta(p.T, d->num_sms);
-  const int grid = route_grid(p.T, d->num_sms);
-  if (grid > 1) {
-    if (!scratch || scratch_bytes < static_cast<size_t>(grid) * p.e_count * sizeof(int)) return BS_ERR_WORKSPACE;
+  if (p.T > bs::kRouteCluster) {
+    if (!scratch || scratch_bytes < static_cast<size_t>(route_grid(p.T, d->num_sms)) * p.e_count * sizeof(int))
+      return BS_ERR_WORKSPACE;
     if (reinterpret_cast<uintptr_t>(scratch) & 3u) return BS_ERR_ALIGN;
     p.hist = static_cast<int*>(scratch);
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (!p.logits) return launch_route<0>(p, 0, grid, s);
-  if (p.E <= 32) return launch_route<1>(p, f32, grid, s);
-  if (p.E <= 64) return launch_route<2>(p, f32, grid, s);
-  if (p.E <= 128) return launch_route<4>(p, f32, grid, s);
-  if (p.E <= 256) return launch_route<8>(p, f32, grid, s);
-  return launch_route<16>(p, f32, grid, s);
+  if (!p.logits) return launch_route<0>(p, 0, d->num_sms, s);
+  if (p.E <= 32) return launch_route<1>(p, f32, d->num_sms, s);
+  if (p.E <= 64) return launch_route<2>(p, f32, d->num_sms, s);
+  if (p.E <= 128) return launch_route<4>(p, f32, d->num_sms, s);
+  if (p.E <= 256) return launch_route<8>(p, f32, d->num_sms, s);
+  return launch_route<16>(p, f32, d->num_sms, s);
 }
 
 // How a grouped product runs.
@@ -226,10 +263,9 @@ int bs_fp8_moe_dispatch(const int* ids, int T, int n_experts, int top_k, int e_b
 }
 
 size_t bs_fp8_moe_scratch_bytes(int T, int e_count) {
-  if (T <= 0 || e_count <= 0) return 0;
+  if (T <= bs::kRouteCluster || e_count <= 0) return 0;
   DeviceState* d = device_state();
-  const int grid = route_grid(T, d ? d->num_sms : 148);
-  return grid > 1 ? static_cast<size_t>(grid) * e_count * sizeof(int) : 0;
+  return static_cast<size_t>(route_grid(T, d ? d->num_sms : 148)) * e_count * sizeof(int);
 }
 
 int bs_fp8_grouped_gemm(const void* A, const void* B, void* C, const float* As, const float* Bs, const int* offsets,

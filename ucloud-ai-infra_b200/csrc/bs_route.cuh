@@ -16,8 +16,9 @@
 // keeps E / 32 logits as ordered integer keys, and a round of the selection is two warp reductions (redux: the
 // maximum, then the lowest index that has it). The plan is a counting sort over CTAs that own contiguous token
 // ranges: k_moe_route ranks each CTA's pairs inside the CTA (match_any inside a warp, a prefix over warps) and leaves
-// its counts per expert, k_moe_place adds the counts of the earlier CTAs and the lower experts. Up to kRouteFuse
-// tokens one CTA does both in one launch. (Ranking in the second kernel instead: 25 us at 8192 tokens, 11.4 at 333.)
+// its counts per expert, k_moe_place adds the counts of the earlier CTAs and the lower experts. (Ranking in the second
+// kernel instead: 25 us at 8192 tokens against 17.) Up to kRouteCluster tokens one launch does both: its CTAs, up to 16,
+// are one cluster and read each other's counts in shared memory.
 #pragma once
 #include "bs_common.cuh"
 
@@ -27,7 +28,8 @@ constexpr int kMaxExperts = 512;
 constexpr int kMaxTopK = 32;
 constexpr int kRouteThreads = 1024;
 constexpr int kRouteWarps = kRouteThreads / 32;
-constexpr int kRouteFuse = 32;   // tokens up to which one CTA counts and places (one round of its 32 warps)
+constexpr int kRouteRound = 32;   // tokens of one round of a CTA's 32 warps
+constexpr int kRouteCluster = 512; // tokens up to which one cluster counts and places in one launch: 16 CTAs, or 8 by two rounds
 constexpr int kRouteBatch = 256; // pairs ranked at a time: 8 warps' counts in shared memory
 constexpr int kRouteRankWarps = kRouteBatch / 32;
 
@@ -45,7 +47,7 @@ struct RouteParams {
   int* offsets;         // [e_count + 1]
   int* row_token;       // [T * k]
   int* slot_row;        // [T, k]
-  int* hist;            // [grid, e_count] counts per CTA (grid > 1)
+  int* hist;            // [grid, e_count] counts per CTA for k_moe_place; nullptr: the grid is one cluster
 };
 
 struct RouteSmem {
@@ -232,11 +234,28 @@ __global__ void __launch_bounds__(kRouteThreads) k_moe_route(const RouteParams p
   const long long n1 = static_cast<long long>(t1) * p.k;
   for (long long b = static_cast<long long>(t0) * p.k; b < n1; b += kRouteBatch) route_rank(sm, p, ids, b, n1);
   __syncthreads();
-  if (gridDim.x > 1) {
+  if (p.hist) {
     if (tid < p.e_count) p.hist[static_cast<size_t>(blockIdx.x) * p.e_count + tid] = sm.count[tid];
     return;
   }
-  route_scan(sm, p, true);
+  if (gridDim.x > 1) {
+    cluster_sync_all();  // every CTA's counts are final
+    int all = 0, before = 0;
+    if (tid < p.e_count)
+      for (uint32_t b = 0; b < gridDim.x; ++b) {
+        int c;
+        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(c) : "r"(mapa_shared(&sm.count[tid], b)) : "memory");
+        all += c;
+        before += b < blockIdx.x ? c : 0;
+      }
+    cluster_sync_all();  // and read by everyone, so they may change and their CTA may end
+    if (tid < p.e_count) {
+      sm.count[tid] = all;
+      sm.base[tid] = before;
+    }
+    __syncthreads();
+  }
+  route_scan(sm, p, blockIdx.x == 0);
   route_place(sm, p, ids, t0, t1);
   route_fill(sm, p);
 }
