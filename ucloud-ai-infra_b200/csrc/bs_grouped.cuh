@@ -131,6 +131,10 @@ __device__ __forceinline__ int source_row(const GroupedParams& p, int r) {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+// 16 bytes of zeros, by the same way.
+__device__ __forceinline__ void cp_async16_zero(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, 0;" ::"r"(dst), "l"(src) : "memory");
+}
 // One arrival on `bar` when every copy this thread has issued so far has landed.
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -289,6 +293,9 @@ __global__ void __launch_bounds__(GroupedRowsCfg<FUSED, BOX>::kThreads, 1)
         mine[lane] = src0;
         mine[lane + 32] = src1;
         __syncwarp();
+        // Rows past the tile's, in sixteens, are zeros, written once into each stage: their results are never read, but
+        // the tensor core's power goes by the values.
+        const int rows = find_tile(table, tile, 128).rows - 64 * w;
         sources(tile + gridDim.x, src0, src1);  // the next tile's, a whole tile ahead
         const uint8_t* src = p.A + c * 16;
         for (int kb = 0; kb < KB; ++kb, src += 128) {
@@ -297,6 +304,13 @@ __global__ void __launch_bounds__(GroupedRowsCfg<FUSED, BOX>::kThreads, 1)
           const uint32_t st = smem_u32(smem + s * Cfg::kStageBytes) + 8192 * w;
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
+            if (4 * i >= rows) {
+              if (kb < S) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) cp_async16_zero(st + ((j & 1) ? odd : even) + 512 * (i + j), src);
+              }
+              continue;
+            }
             const uint4 o = *reinterpret_cast<const uint4*>(mine + 16 * sub + i);
             cp_async16(st + even + 512 * i, src + static_cast<uint64_t>(o.x) * 16);
             cp_async16(st + odd + 512 * (i + 1), src + static_cast<uint64_t>(o.y) * 16);
