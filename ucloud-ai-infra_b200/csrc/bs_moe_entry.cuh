@@ -91,10 +91,10 @@ struct GroupedPlan {
 
 // Chosen by the mean rows per expert. Measured with router-like skew (times in us; 64 experts, 5120 -> 2 x 1024 fused,
 // 1024 -> 5120 plain; 128 experts, 2048 -> 2 x 768, 768 -> 2048; token tiles of 16 and 32 rows, row tiles):
-//   fused  mean 4.0: 97.8, 98.3, 129 (64 experts)    4.7: 58.7, 57.3, 75.8 (128)    7.6: 106, 101, 135 (64)
-//          mean 18.8: 103, 86.4, 84.8 (128)   20: 153, 127, 137 (64)   30: 209, 160, 138 (64)
-//   plain  mean 4.0: 53.0, 54.4, 57.4 (64)    4.7: 38.3, 35.6, 38.0 (128)   11.2: 50.0, 43.7, 44.2 (128)
-//          mean 12.5: 74.3, 64.0, 65.6 (64)   18.8: 65.7, 49.9, 44.9 (128)  20: 96.5, 72.4, 66.7 (64)
+//   fused  mean 4.0: 97.8, 98.3, 125 (64 experts)    4.7: 58.7, 57.3, 72 (128)    12.5: -, 111, 125 (64)
+//          mean 14.1: -, 76.3, 76.6 (128)   17.5: -, 115, 127 (64)   19.7: -, 88.5, 81.6 (128)   20: -, 127, 127 (64)
+//   plain  mean 4.0: 53.0, 54.4, 57.4 (64)   4.7: 38.3, 35.6, 38.0 (128)   12.5: -, 63.6, 66.9 (64)
+//          mean 14.1: -, 44.7, 44.1 (128)    15: -, 67.4, 67.1 (64)        17.5: -, 69.2, 67.7 (64)
 // (token tiles of 64 rows were never more than 1 us ahead of the better of 32 and row tiles: not built).
 // CTAs per tile: a call with fewer tiles than SMs takes as many as fill them, with at least 8 K blocks each (36 tiles of
 // 16 K blocks: 14.6 us on one CTA each, 11.2 on two, 12.0 on four; 64 tiles of 40: 27.7, 19.3, 19.4). With more
@@ -104,7 +104,7 @@ GroupedPlan grouped_plan(bool fused, int E, int nblk, int KB, int rows, int num_
   GroupedPlan g = {0, 0};
   const long long r = rows;
   if (r <= 4ll * E) g.nt = 16;
-  else if (r <= (fused ? 18ll : 14ll) * E) g.nt = 32;
+  else if (r <= (fused ? 16ll : 14ll) * E) g.nt = 32;
   if (!g.nt) return g;
   const long long tiles = static_cast<long long>(rows < E ? rows : E) * (fused ? nblk / 2 : nblk);
   if (tiles > num_sms)
