@@ -73,18 +73,21 @@ __host__ __device__ inline BlockRing block_ring(int k, int H, int res_bytes) {
 // The widest: fp32 residual rows and one-row stages of kBlockMaxH elements.
 constexpr int kBlockMaxSmem = kBlockResSlots * 4 * kBlockMaxH + 2 * 2 * kBlockMaxH;
 
-// Sum over the `threads` consumer threads in a fixed order: a butterfly per warp, then one over the (at most 16) warp totals.
-// `buf` is not reused before the next barrier.
-__device__ __forceinline__ float block_sum(float v, float* buf, int threads) {
+// Sum over the `threads` consumer threads in a fixed order, in two halves so that other work can stand between them: a
+// butterfly per warp and its total in `buf`; then, after the barrier, a butterfly over the (at most 16) warp totals. `buf`
+// is not reused before the next barrier.
+__device__ __forceinline__ void block_sum_begin(float v, float* buf) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  const int lane = threadIdx.x & 31;
-  if (lane == 0) buf[threadIdx.x >> 5] = v;
+  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
+}
+__device__ __forceinline__ float block_sum_end(const float* buf, int threads) {
   named_bar_sync(1, threads);
-  float s = lane < (threads >> 5) ? buf[lane] : 0.f;
+  const int i = threadIdx.x & 15;
+  float s = i < (threads >> 5) ? buf[i] : 0.f;
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  return __shfl_sync(0xffffffffu, s, 0);
+  return s;
 }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
@@ -275,26 +278,38 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
         ph ^= 1;
       }
     }
-    auto square_sum = [&](float* buf) {
+    auto squares = [&]() {
       uint64_t ss2 = 0;
 #pragma unroll
       for (int j = 0; j < C; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) ss2 = ffma2r(z[j][e], z[j][e], ss2);  // zero past the row's end
-      const float ss = block_sum(lo_f(ss2) + hi_f(ss2), buf, nt);
-      return rsqrtf(fmaf(ss, p.inv_h, p.eps));
+      return lo_f(ss2) + hi_f(ss2);
     };
+    // The gate's chunks are on the way during the first reduction, the next norm's weight during what follows it.
+    uint4 g4[C];
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      if constexpr (kKeep) g4[j] = gv[j];
+      else g4[j] = chunk(p.gate_kind == kGateFull ? p.gate + row * p.ldg : channel, t + nt * j);
+    }
     if (p.post) {
-      const float rs = square_sum(sums[parity][0]);
+      uint4 w4[C];
+#pragma unroll
+      for (int j = 0; j < C; ++j) w4[j] = kKeep ? post[kKeep ? j : 0] : chunk(p.post, t + nt * j);
+      block_sum_begin(squares(), sums[parity][0]);
+      const float rs = rsqrtf(fmaf(block_sum_end(sums[parity][0], nt), p.inv_h, p.eps));
       const uint64_t rs2 = pack_f2(rs, rs);
 #pragma unroll
       for (int j = 0; j < C; ++j) {
-        const uint4 wv = kKeep ? post[kKeep ? j : 0] : chunk(p.post, t + nt * j);
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(&wv);
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&w4[j]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) z[j][e] = fmul2(fmul2(z[j][e], rs2), bf16x2_to_f2(w[e]));
       }
     }
+    uint4 next[C];
+#pragma unroll
+    for (int j = 0; j < C; ++j) next[j] = kKeep ? pre[kKeep ? j : 0] : chunk(p.pre, t + nt * j);
     if (res_bytes && ok) ok = mbar_wait_warp(&rfull[rs], rph, &abort_flag, p.status, kErrTimeoutFull);
     const uint4* res = reinterpret_cast<const uint4*>(block_smem + rs * res_bytes);
     const uint64_t gs2 = pack_f2(gt, gt), a2 = pack_f2(p.residual_scale, p.residual_scale);
@@ -302,10 +317,7 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
     for (int j = 0; j < C; ++j) {
       const int c = t + nt * j;
       if (c < nch) {
-        uint4 g4;
-        if constexpr (kKeep) g4 = gv[j];
-        else g4 = chunk(p.gate_kind == kGateFull ? p.gate + row * p.ldg : channel, c);
-        const uint32_t* gw = reinterpret_cast<const uint32_t*>(&g4);
+        const uint32_t* gw = reinterpret_cast<const uint32_t*>(&g4[j]);
         uint4 rv[WIDE ? 2 : 1];
 #pragma unroll
         for (int i = 0; i < (WIDE ? 2 : 1); ++i) rv[i] = res_bytes && ok ? res[WIDE ? 2 * c + i : c] : make_uint4(0, 0, 0, 0);
@@ -345,49 +357,54 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
       }
     }
     if (p.pre) {
-      // v = u * rs with u = h * pre. The quotient v / As is u / (amax(u) / 448), so the row's 1 / sqrt only enters As,
-      // and the bytes see one rounding (of u) before the division; rows so small that As is at its floor divide
-      // u * rs by the floor.
-      const float rs = square_sum(sums[parity][1]);
+      // v = u * rs with u = h * pre. The quotient v / As is u / (amax(u) / 448), so the row's 1 / sqrt only enters As:
+      // the bytes are made while the sum is on its way, and see one rounding (of u) before the division. Groups so
+      // small that As is at its floor divide u * rs by the floor instead.
+      block_sum_begin(squares(), sums[parity][1]);
+      uint32_t q[C][2];
+      float su[C];
+      auto quant = [&](const uint64_t (&u)[4], float div, float mul, uint32_t (&out)[2]) {
+        const float nr = -__frcp_rn(div);
+        const uint64_t d2 = pack_f2(div, div), nr2 = pack_f2(nr, nr), m2 = pack_f2(mul, mul);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint64_t q0 = neg_div_by_scale2(fmul2(u[2 * h], m2), d2, nr2);
+          const uint64_t q1 = neg_div_by_scale2(fmul2(u[2 * h + 1], m2), d2, nr2);
+          out[h] = (f2_to_e4m3x2(lo_f(q0), hi_f(q0)) | (f2_to_e4m3x2(lo_f(q1), hi_f(q1)) << 16)) ^ 0x80808080u;
+        }
+      };
 #pragma unroll
       for (int j = 0; j < C; ++j) {
-        if (nt * j >= nch) break;  // uniform across the CTA
-        const int c = t + nt * j;
-        const uint4 wv = kKeep ? pre[kKeep ? j : 0] : chunk(p.pre, c);
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(&wv);
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&next[j]);
         float amax = 0.f;
-        uint64_t u[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          u[e] = fmul2(z[j][e], bf16x2_to_f2(w[e]));
-          amax = fmaxf(amax, fmaxf(fabsf(lo_f(u[e])), fabsf(hi_f(u[e]))));
+          z[j][e] = fmul2(z[j][e], bf16x2_to_f2(w[e]));  // u
+          amax = fmaxf(amax, fmaxf(fabsf(lo_f(z[j][e])), fabsf(hi_f(z[j][e]))));
         }
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        const float su = amax_div_448(amax);
-        float as = __fmul_rn(su, rs), div = su, mul = 1.0f;
+        su[j] = amax_div_448(amax);
+        quant(z[j], su[j], 1.0f, q[j]);
+      }
+      const float rs = rsqrtf(fmaf(block_sum_end(sums[parity][1], nt), p.inv_h, p.eps));
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        const int c = t + nt * j;
+        float as = __fmul_rn(su[j], rs);
         if (!(as >= 1e-12f)) {
-          as = div = 1e-12f;
-          mul = rs;
+          as = 1e-12f;
+          quant(z[j], as, rs, q[j]);
         }
         if (c < nch && ok) {
-          const float nr = -__frcp_rn(div);
-          const uint64_t d2 = pack_f2(div, div), nr2 = pack_f2(nr, nr), m2 = pack_f2(mul, mul);
-          uint32_t q[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint64_t q0 = neg_div_by_scale2(fmul2(u[2 * h], m2), d2, nr2);
-            const uint64_t q1 = neg_div_by_scale2(fmul2(u[2 * h + 1], m2), d2, nr2);
-            q[h] = (f2_to_e4m3x2(lo_f(q0), hi_f(q0)) | (f2_to_e4m3x2(lo_f(q1), hi_f(q1)) << 16)) ^ 0x80808080u;
-          }
-          *reinterpret_cast<uint2*>(p.A + static_cast<size_t>(row) * p.H + c * 8) = make_uint2(q[0], q[1]);
+          *reinterpret_cast<uint2*>(p.A + static_cast<size_t>(row) * p.H + c * 8) = make_uint2(q[j][0], q[j][1]);
           if ((lane & 15) == 0) p.As[static_cast<size_t>(row) * (p.H / 128) + c / 16] = as;
           if (p.V) {
             const uint64_t rs2 = pack_f2(rs, rs);
             uint32_t v[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const uint64_t x = fmul2(u[e], rs2);
+              const uint64_t x = fmul2(z[j][e], rs2);
               v[e] = pack_bf16x2(lo_f(x), hi_f(x));
             }
             *reinterpret_cast<uint4*>(p.V + static_cast<size_t>(row) * p.H + c * 8) = make_uint4(v[0], v[1], v[2], v[3]);
