@@ -12,7 +12,7 @@
 // Two kernels (the choice between them, with both measured: grouped_plan in bs_moe_entry.cuh).
 //   k_grouped_rows    128 rows x 256 weight columns per tile, rows on the MMA's 128 lanes, for experts with many rows. Bound
 //                     by the promotion of each K block's partial and by power: 8192 tokens x 8 of 64 experts, fused
-//                     5120 -> 2 x 1024 880 us, plain 1024 -> 5120 483 us (1.5 PFLOP/s, at 1.45-1.65 GHz under the
+//                     5120 -> 2 x 1024 858 us, plain 1024 -> 5120 475 us (1.5 PFLOP/s, at 1.45-1.65 GHz under the
 //                     1000 W limit; a tile costs 128 rows whatever it holds)
 //   k_grouped_tokens  128 weight rows on the lanes, up to 16 or 32 rows on the columns, for experts with few rows. Bound by
 //                     the weights' stream: 61 tokens x 8 of 64 experts, the same products: 101 us (6.65 TB/s), 58 us;
@@ -598,7 +598,8 @@ struct GroupedTokensCfg {
   static constexpr int kBlockBytes = kWBytes + ((kXBytes + 1023) / 1024) * 1024;
   static constexpr int kStageBytes = kKu * kBlockBytes;
   static constexpr int kBufCols = kSets * NT;
-  static constexpr int kBufs = 512 / kBufCols > 4 ? 4 : 512 / kBufCols;
+  // 4 and 8 buffers: 69.0 and 67.5 us where a CTA has several tiles (fused, 128 experts, 160 tokens), equal elsewhere.
+  static constexpr int kBufs = 8;
   static constexpr int kTmemCols = kBufs * kBufCols;
   static_assert((kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols >= 32 && kTmemCols <= 512, "TMEM columns");
   static constexpr int kSlots = 8;
@@ -1033,7 +1034,9 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
         }
       }
       if (ok && log_s > 0) {
-        // This warp's reads are done (their values are in the stores above): the count alone is enough.
+        // This warp's reads are done: each value read went into a store above, so no load is still under way when the
+        // arrival issues, and the count alone is enough. (A releasing arrival also waits for those stores to reach
+        // global memory: 61 tokens 101.0 -> 104.2 us, 128 experts and 160 tokens 67.5 -> 78.2.)
         __syncwarp();
         if (lane < S) mbar_arrive_remote_relaxed(mapa_shared(rempty, lane));
       }
