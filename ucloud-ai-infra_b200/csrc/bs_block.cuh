@@ -73,9 +73,10 @@ __host__ __device__ inline BlockRing block_ring(int k, int H, int res_bytes) {
 // The widest: fp32 residual rows and one-row stages of kBlockMaxH elements.
 constexpr int kBlockMaxSmem = kBlockResSlots * 4 * kBlockMaxH + 2 * 2 * kBlockMaxH;
 
+constexpr int kBlockSums = (kBlockMaxThreads / 32 + 3) / 4 * 4;  // warp totals; those of warps that do not exist are 0
 // Sum over the `threads` consumer threads in a fixed order, in two halves so that other work can stand between them: a
-// butterfly per warp and its total in `buf`; then, after the barrier, a butterfly over the (at most 16) warp totals. `buf`
-// is not reused before the next barrier.
+// butterfly per warp and its total in `buf`; then, after the barrier, every thread adds the warp totals. `buf` is not
+// reused before the next barrier.
 __device__ __forceinline__ void block_sum_begin(float v, float* buf) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -83,11 +84,11 @@ __device__ __forceinline__ void block_sum_begin(float v, float* buf) {
 }
 __device__ __forceinline__ float block_sum_end(const float* buf, int threads) {
   named_bar_sync(1, threads);
-  const int i = threadIdx.x & 15;
-  float s = i < (threads >> 5) ? buf[i] : 0.f;
+  const ulonglong2* b = reinterpret_cast<const ulonglong2*>(buf);
+  uint64_t s = fadd2(b[0].x, b[0].y);
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  return s;
+  for (int i = 1; i < kBlockSums / 4; ++i) s = fadd2(s, fadd2(b[i].x, b[i].y));
+  return lo_f(s) + hi_f(s);
 }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
@@ -109,7 +110,7 @@ __device__ __forceinline__ float amax_div_448(float amax) {
 template <int C, bool WIDE>
 __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block_norm(const BlockParams p) {
   extern __shared__ __align__(128) uint8_t block_smem[];  // residual rows, then [stages][G rows][2 H]
-  __shared__ float sums[2][2][kBlockMaxThreads / 32];  // by row parity and norm
+  __shared__ __align__(16) float sums[2][2][kBlockSums];  // by row parity and norm
   __shared__ uint64_t full[kBlockMaxStages], empty[kBlockMaxStages];
   __shared__ uint64_t rfull[kBlockResSlots], rempty[kBlockResSlots];
   __shared__ float4 weight[kBlockMaxStages];
@@ -121,6 +122,8 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
   const BlockRing br = block_ring(k, p.H, p.residual ? (WIDE ? 4 : 2) * p.H : 0);
   const int G = br.G, stages = br.stages, res_bytes = br.res_bytes;
   uint8_t* ring = block_smem + kBlockResSlots * res_bytes;
+  static_assert(sizeof(sums) / 4 <= 64, "two warps at least");
+  if (t < static_cast<int>(sizeof(sums) / 4)) (&sums[0][0][0])[t] = 0.f;
   if (t == 0) {
     for (int i = 0; i < stages; ++i) {
       mbar_init(&full[i], 2);  // both by the producer: the bytes to come, and the weights
@@ -211,33 +214,17 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
   }
 
   // -------------------------------------------------------------- rows
-  // What every row uses, the norm weights' and a channel gate's chunks of this thread, stays in registers where a
-  // thread has one chunk; wider rows read it again (from L1), and two CTAs fit on an SM.
-  constexpr bool kKeep = C <= 1;
-  uint4 post[kKeep ? C : 1], pre[kKeep ? C : 1], gch[kKeep ? C : 1];
+  // What every row uses, the norm weights' and a channel gate's chunks of this thread, is read again for each row (from
+  // L1), always ahead of a reduction: kept in registers it spills (8192 x 2560, one chunk a thread, k = 8: 83 us, 78 so).
   auto chunk = [&](const __nv_bfloat16* w, int c) {
     return w && c < nch ? __ldg(reinterpret_cast<const uint4*>(w + c * 8)) : make_uint4(0, 0, 0, 0);
   };
   const __nv_bfloat16* channel = p.gate_kind == kGateChannel ? p.gate : nullptr;
-  if constexpr (kKeep) {
-#pragma unroll
-    for (int j = 0; j < C; ++j) {
-      post[j] = chunk(p.post, t + nt * j);
-      pre[j] = chunk(p.pre, t + nt * j);
-      gch[j] = chunk(channel, t + nt * j);
-    }
-  }
   int st = 0, rs = 0;
   uint32_t ph = 0, rph = 0;
   bool ok = true;
   for (int row = blockIdx.x, parity = 0; row < p.T; row += gridDim.x, parity ^= 1) {
-    // in flight while the rows are added up
-    uint4 gv[kKeep ? C : 1];
     float gt = p.scale;
-    if constexpr (kKeep) {
-#pragma unroll
-      for (int j = 0; j < C; ++j) gv[j] = p.gate_kind == kGateFull ? chunk(p.gate + row * p.ldg, t + nt * j) : gch[j];
-    }
     if (p.gate_kind == kGateToken) gt = __bfloat162float(__ldg(p.gate + row * p.ldg)) * p.scale;
 
     uint64_t z[C][4];  // pairs of this thread's elements
@@ -245,6 +232,13 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
     for (int j = 0; j < C; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) z[j][e] = 0;
+    auto add = [&](int j, const uint4& v, float w) {
+      const uint64_t w2 = pack_f2(w, w);
+      z[j][0] = ffma2r(w2, bf16x2_to_f2(v.x), z[j][0]);
+      z[j][1] = ffma2r(w2, bf16x2_to_f2(v.y), z[j][1]);
+      z[j][2] = ffma2r(w2, bf16x2_to_f2(v.z), z[j][2]);
+      z[j][3] = ffma2r(w2, bf16x2_to_f2(v.w), z[j][3]);
+    };
     for (int s = 0; s < k; s += G) {
       if (ok) ok = mbar_wait_warp(&full[st], ph, &abort_flag, p.status, kErrTimeoutFull);
       if (ok) {
@@ -255,19 +249,17 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
 #pragma unroll
         for (int j = 0; j < C; ++j) {
           if (t + nt * j < nch) {
+            if (G == 1) {
+              if (mask) add(j, *reinterpret_cast<const uint4*>(src + nt * j * 16), w4.x);
+              continue;
+            }
             uint4 v[4];
 #pragma unroll
             for (int g = 0; g < 4; ++g)
               if ((mask >> g) & 1) v[g] = *reinterpret_cast<const uint4*>(src + g * row_bytes + nt * j * 16);
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-              if ((mask >> g) & 1) {
-                const uint64_t w2 = pack_f2(w[g], w[g]);
-                z[j][0] = ffma2r(w2, bf16x2_to_f2(v[g].x), z[j][0]);
-                z[j][1] = ffma2r(w2, bf16x2_to_f2(v[g].y), z[j][1]);
-                z[j][2] = ffma2r(w2, bf16x2_to_f2(v[g].z), z[j][2]);
-                z[j][3] = ffma2r(w2, bf16x2_to_f2(v[g].w), z[j][3]);
-              }
+              if ((mask >> g) & 1) add(j, v[g], w[g]);
           }
         }
       }
@@ -289,14 +281,11 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
     // The gate's chunks are on the way during the first reduction, the next norm's weight during what follows it.
     uint4 g4[C];
 #pragma unroll
-    for (int j = 0; j < C; ++j) {
-      if constexpr (kKeep) g4[j] = gv[j];
-      else g4[j] = chunk(p.gate_kind == kGateFull ? p.gate + row * p.ldg : channel, t + nt * j);
-    }
+    for (int j = 0; j < C; ++j) g4[j] = chunk(p.gate_kind == kGateFull ? p.gate + row * p.ldg : channel, t + nt * j);
     if (p.post) {
       uint4 w4[C];
 #pragma unroll
-      for (int j = 0; j < C; ++j) w4[j] = kKeep ? post[kKeep ? j : 0] : chunk(p.post, t + nt * j);
+      for (int j = 0; j < C; ++j) w4[j] = chunk(p.post, t + nt * j);
       block_sum_begin(squares(), sums[parity][0]);
       const float rs = rsqrtf(fmaf(block_sum_end(sums[parity][0], nt), p.inv_h, p.eps));
       const uint64_t rs2 = pack_f2(rs, rs);
@@ -309,7 +298,7 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
     }
     uint4 next[C];
 #pragma unroll
-    for (int j = 0; j < C; ++j) next[j] = kKeep ? pre[kKeep ? j : 0] : chunk(p.pre, t + nt * j);
+    for (int j = 0; j < C; ++j) next[j] = chunk(p.pre, t + nt * j);
     if (res_bytes && ok) ok = mbar_wait_warp(&rfull[rs], rph, &abort_flag, p.status, kErrTimeoutFull);
     const uint4* res = reinterpret_cast<const uint4*>(block_smem + rs * res_bytes);
     const uint64_t gs2 = pack_f2(gt, gt), a2 = pack_f2(p.residual_scale, p.residual_scale);
@@ -363,13 +352,13 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
       block_sum_begin(squares(), sums[parity][1]);
       uint32_t q[C][2];
       float su[C];
-      auto quant = [&](const uint64_t (&u)[4], float div, float mul, uint32_t (&out)[2]) {
+      auto quant = [&](const uint64_t (&u)[4], float div, uint32_t (&out)[2]) {
         const float nr = -__frcp_rn(div);
-        const uint64_t d2 = pack_f2(div, div), nr2 = pack_f2(nr, nr), m2 = pack_f2(mul, mul);
+        const uint64_t d2 = pack_f2(div, div), nr2 = pack_f2(nr, nr);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint64_t q0 = neg_div_by_scale2(fmul2(u[2 * h], m2), d2, nr2);
-          const uint64_t q1 = neg_div_by_scale2(fmul2(u[2 * h + 1], m2), d2, nr2);
+          const uint64_t q0 = neg_div_by_scale2(u[2 * h], d2, nr2);
+          const uint64_t q1 = neg_div_by_scale2(u[2 * h + 1], d2, nr2);
           out[h] = (f2_to_e4m3x2(lo_f(q0), hi_f(q0)) | (f2_to_e4m3x2(lo_f(q1), hi_f(q1)) << 16)) ^ 0x80808080u;
         }
       };
@@ -382,10 +371,12 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
           z[j][e] = fmul2(z[j][e], bf16x2_to_f2(w[e]));  // u
           amax = fmaxf(amax, fmaxf(fabsf(lo_f(z[j][e])), fabsf(hi_f(z[j][e]))));
         }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        su[j] = amax_div_448(amax);
-        quant(z[j], su[j], 1.0f, q[j]);
+        // of this half-warp: never NaN, and floats from 0 up order like their bits
+        const uint32_t bits = __float_as_uint(amax);
+        const uint32_t lo = __reduce_max_sync(0xffffffffu, lane < 16 ? bits : 0u);
+        const uint32_t hi = __reduce_max_sync(0xffffffffu, lane < 16 ? 0u : bits);
+        su[j] = amax_div_448(__uint_as_float(lane < 16 ? lo : hi));
+        quant(z[j], su[j], q[j]);
       }
       const float rs = rsqrtf(fmaf(block_sum_end(sums[parity][1], nt), p.inv_h, p.eps));
 #pragma unroll
@@ -394,7 +385,10 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
         float as = __fmul_rn(su[j], rs);
         if (!(as >= 1e-12f)) {
           as = 1e-12f;
-          quant(z[j], as, rs, q[j]);
+          uint64_t v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = fmul2(z[j][e], pack_f2(rs, rs));
+          quant(v, as, q[j]);
         }
         if (c < nch && ok) {
           *reinterpret_cast<uint2*>(p.A + static_cast<size_t>(row) * p.H + c * 8) = make_uint2(q[j][0], q[j][1]);
