@@ -255,6 +255,32 @@ def test_block_norm(cuda_lib, T, H, k, wide, gate):
     _check_block(out, (want[0], want[1], None, None), wide)
 
 
+@pytest.mark.parametrize("T,H,k,wide", [(320, 2560, 4, False), (310, 2688, 1, True), (301, 5248, 8, False),
+                                        (160, 7168, 5, True), (170, 10240, 0, False), (150, 10368, 2, True),
+                                        (151, 16384, 8, True)])
+def test_block_row_lengths(cuda_lib, T, H, k, wide):
+    """The first and last lengths of the kernel's shapes, with several rows per CTA."""
+    y, res, post, pre, w, slot, g = _block_case(T, H, k, wide, T + H + k)
+    gt = torch.sigmoid(torch.randn(H, generator=g)).to(torch.bfloat16)
+    kw = dict(scale=0.9, residual_scale=1.1, eps=1e-6)
+    got = _ops().block_norm_quant(y.cuda(), res.cuda(), post_weight=post.cuda(), gate=gt.cuda(), pre_weight=pre.cuda(),
+                                  route=_route_of(w, slot), **kw)
+    _check_block(got, M.block(y, res, post=post, gate=gt, pre=pre, weights=w, slot_row=slot, **kw), wide)
+
+
+@pytest.mark.parametrize("H", [640, 5120, 8192])
+def test_block_scales_at_their_floor(cuda_lib, H):
+    """Groups whose norm weight is so small that the scale is at its floor beside ordinary ones."""
+    y, res, post, pre, _, _, _ = _block_case(7, H, 0, False, H)
+    pre[:128] *= 1e-13
+    pre[256:384] = 0
+    pre[384:512] *= 1e-30
+    got = _ops().block_norm_quant(y.cuda(), res.cuda(), post_weight=post.cuda(), pre_weight=pre.cuda())
+    _check_block(got, M.block(y, res, post=post, pre=pre), False)
+    floor = got[2] == torch.tensor(1e-12)
+    assert bool(floor[:, [0, 2, 3]].all()) and not bool(floor[:, [1, 4]].any())
+
+
 @pytest.mark.parametrize("k", [0, 4])
 def test_block_plain_add_and_norm(cuda_lib, k):
     """No norm after the block and no gate: h = residual + z, then the next block's quant."""

@@ -22,7 +22,6 @@
 
 namespace bs {
 
-constexpr int kBlockMaxThreads = 320;  // that own chunks, beside the producer warp
 constexpr int kBlockMaxH = 16384;
 
 enum : int { kGateNone = 0, kGateChannel = 1, kGateToken = 2, kGateFull = 3 };
@@ -53,27 +52,40 @@ struct BlockParams {
 };
 
 constexpr int kBlockMaxStages = 16;
-constexpr int kBlockRingBytes = 100 * 1024;  // two CTAs per SM
 
 constexpr int kBlockResSlots = 2;
+
+// Shapes of the kernel: chunks per thread, most threads that own chunks (a producer warp comes on top), CTAs per SM that
+// its registers and its ring leave room for. By the row's length: two small CTAs overlap one's reductions with the other's
+// reads; rows too long for them have one large CTA rather than more chunks a thread (T = 8192, k = 8, us; two chunks of
+// 640 threads against four chunks of 320: H = 6144 190 and 306, 8192 221 and 349).
+template <int C_, int THREADS, int CTAS>
+struct BlockShape {
+  static constexpr int C = C_, kThreads = THREADS, kCtas = CTAS;
+  static constexpr int kMaxH = C * THREADS * 8;
+  static constexpr int kRingBytes = 200 * 1024 / CTAS;
+  static constexpr int kSums = (THREADS / 32 + 3) / 4 * 4;  // warp totals; those of warps that do not exist are 0
+  static_assert(kBlockResSlots * 4 * kMaxH + 2 * 2 * kMaxH <= kRingBytes, "fp32 residual rows and two stages");
+};
+using BlockShape1 = BlockShape<1, 320, 2>;
+using BlockShape2 = BlockShape<2, 320, 2>;
+using BlockShape3 = BlockShape<2, 640, 1>;
+using BlockShape4 = BlockShape<4, 512, 1>;
+static_assert(BlockShape4::kMaxH == kBlockMaxH, "every row has a shape");
 
 // The ring of a launch: two residual rows, and stages of G rows (a power of two), two at least.
 struct BlockRing {
   int G, stages, res_bytes;  // res_bytes: a residual row's, 0 without one
   __host__ __device__ int bytes(int H) const { return kBlockResSlots * res_bytes + stages * G * 2 * H; }
 };
-__host__ __device__ inline BlockRing block_ring(int k, int H, int res_bytes) {
+__host__ __device__ inline BlockRing block_ring(int k, int H, int res_bytes, int ring_bytes) {
   BlockRing r = {k >= 3 ? 4 : k, 0, res_bytes};
-  const int room = kBlockRingBytes - kBlockResSlots * res_bytes;
+  const int room = ring_bytes - kBlockResSlots * res_bytes;
   while (r.G > 1 && 2 * r.G * 2 * H > room) r.G >>= 1;
   const int n = room / (r.G * 2 * H);
   r.stages = n < 2 ? 2 : n > kBlockMaxStages ? kBlockMaxStages : n;
   return r;
 }
-// The widest: fp32 residual rows and one-row stages of kBlockMaxH elements.
-constexpr int kBlockMaxSmem = kBlockResSlots * 4 * kBlockMaxH + 2 * 2 * kBlockMaxH;
-
-constexpr int kBlockSums = (kBlockMaxThreads / 32 + 3) / 4 * 4;  // warp totals; those of warps that do not exist are 0
 // Sum over the `threads` consumer threads in a fixed order, in two halves so that other work can stand between them: a
 // butterfly per warp and its total in `buf`; then, after the barrier, every thread adds the warp totals. `buf` is not
 // reused before the next barrier.
@@ -82,12 +94,13 @@ __device__ __forceinline__ void block_sum_begin(float v, float* buf) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
 }
-__device__ __forceinline__ float block_sum_end(const float* buf, int threads) {
+template <int SUMS>
+__device__ __forceinline__ float block_sum_end(const float (&buf)[SUMS], int threads) {
   named_bar_sync(1, threads);
   const ulonglong2* b = reinterpret_cast<const ulonglong2*>(buf);
   uint64_t s = fadd2(b[0].x, b[0].y);
 #pragma unroll
-  for (int i = 1; i < kBlockSums / 4; ++i) s = fadd2(s, fadd2(b[i].x, b[i].y));
+  for (int i = 1; i < SUMS / 4; ++i) s = fadd2(s, fadd2(b[i].x, b[i].y));
   return lo_f(s) + hi_f(s);
 }
 
@@ -107,10 +120,11 @@ __device__ __forceinline__ float amax_div_448(float amax) {
   return __fmaf_rn(__fmaf_rn(-448.0f, q0, amax), kInv448, q0);
 }
 
-template <int C, bool WIDE>
-__global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block_norm(const BlockParams p) {
+template <typename Shape, bool WIDE>
+__global__ void __launch_bounds__(Shape::kThreads + 32, Shape::kCtas) k_block_norm(const BlockParams p) {
+  constexpr int C = Shape::C;
   extern __shared__ __align__(128) uint8_t block_smem[];  // residual rows, then [stages][G rows][2 H]
-  __shared__ __align__(16) float sums[2][2][kBlockSums];  // by row parity and norm
+  __shared__ __align__(16) float sums[2][2][Shape::kSums];  // by row parity and norm
   __shared__ uint64_t full[kBlockMaxStages], empty[kBlockMaxStages];
   __shared__ uint64_t rfull[kBlockResSlots], rempty[kBlockResSlots];
   __shared__ float4 weight[kBlockMaxStages];
@@ -119,11 +133,10 @@ __global__ void __launch_bounds__(kBlockMaxThreads + 32, C <= 2 ? 2 : 1) k_block
   const int t = threadIdx.x, nt = static_cast<int>(blockDim.x) - 32, lane = t & 31;
   const int nch = p.H / 8, row_bytes = 2 * p.H;
   const int k = p.weights ? p.k : 1;
-  const BlockRing br = block_ring(k, p.H, p.residual ? (WIDE ? 4 : 2) * p.H : 0);
+  const BlockRing br = block_ring(k, p.H, p.residual ? (WIDE ? 4 : 2) * p.H : 0, Shape::kRingBytes);
   const int G = br.G, stages = br.stages, res_bytes = br.res_bytes;
   uint8_t* ring = block_smem + kBlockResSlots * res_bytes;
-  static_assert(sizeof(sums) / 4 <= 64, "two warps at least");
-  if (t < static_cast<int>(sizeof(sums) / 4)) (&sums[0][0][0])[t] = 0.f;
+  for (int i = t; i < 4 * Shape::kSums; i += blockDim.x) (&sums[0][0][0])[i] = 0.f;
   if (t == 0) {
     for (int i = 0; i < stages; ++i) {
       mbar_init(&full[i], 2);  // both by the producer: the bytes to come, and the weights

@@ -195,12 +195,14 @@ bs::GroupedParams grouped_params(const void* A, const float* As, const float* Bs
   return p;
 }
 
-template <int C, bool WIDE>
-int launch_block(const bs::BlockParams& p, int threads, int num_sms, cudaStream_t s) {
-  constexpr auto kern = bs::k_block_norm<C, WIDE>;
-  const int rc = prepare_kernel<kern>(bs::kBlockMaxSmem, 0);
+template <typename Shape, bool WIDE>
+int launch_block(const bs::BlockParams& p, int num_sms, cudaStream_t s) {
+  constexpr auto kern = bs::k_block_norm<Shape, WIDE>;
+  const int res_bytes = p.residual ? (WIDE ? 4 : 2) * p.H : 0;
+  const int smem = bs::block_ring(p.weights ? p.k : 1, p.H, res_bytes, Shape::kRingBytes).bytes(p.H);
+  const int rc = prepare_kernel<kern>(Shape::kRingBytes, 0);
   if (rc != BS_OK) return rc;
-  const int smem = bs::block_ring(p.weights ? p.k : 1, p.H, p.residual ? (WIDE ? 4 : 2) * p.H : 0).bytes(p.H);
+  const int threads = ((p.H / 8 + Shape::C - 1) / Shape::C + 31) / 32 * 32;
   int grid = p.T;  // a CTA per token, or as many as fit
   if (p.T > num_sms) {
     int per_sm = 0;
@@ -212,9 +214,9 @@ int launch_block(const bs::BlockParams& p, int threads, int num_sms, cudaStream_
   return launch_pdl(kern, grid, threads + 32, smem, s, "k_block_norm launch", p);
 }
 
-template <int C>
-int launch_block_c(const bs::BlockParams& p, bool wide, int threads, int num_sms, cudaStream_t s) {
-  return wide ? launch_block<C, true>(p, threads, num_sms, s) : launch_block<C, false>(p, threads, num_sms, s);
+template <typename Shape>
+int launch_block_shape(const bs::BlockParams& p, bool wide, int num_sms, cudaStream_t s) {
+  return wide ? launch_block<Shape, true>(p, num_sms, s) : launch_block<Shape, false>(p, num_sms, s);
 }
 
 }  // namespace
@@ -342,17 +344,12 @@ int bs_fp8_block_norm_quant(const void* y, long long ldy, int rows_y, const floa
   p.V = static_cast<__nv_bfloat16*>(V);
   p.T = T;
   p.H = H;
-  const int chunks = H / 8;
-  const int c = chunks <= bs::kBlockMaxThreads ? 1 : chunks <= 2 * bs::kBlockMaxThreads ? 2 : chunks <= 4 * bs::kBlockMaxThreads ? 4 : 7;
-  const int threads = ((chunks + c - 1) / c + 31) / 32 * 32;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   p.status = d->status;
-  switch (c) {
-    case 1: return launch_block_c<1>(p, wide != 0, threads, d->num_sms, s);
-    case 2: return launch_block_c<2>(p, wide != 0, threads, d->num_sms, s);
-    case 4: return launch_block_c<4>(p, wide != 0, threads, d->num_sms, s);
-    default: return launch_block_c<7>(p, wide != 0, threads, d->num_sms, s);
-  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (H <= bs::BlockShape1::kMaxH) return launch_block_shape<bs::BlockShape1>(p, wide != 0, d->num_sms, s);
+  if (H <= bs::BlockShape2::kMaxH) return launch_block_shape<bs::BlockShape2>(p, wide != 0, d->num_sms, s);
+  if (H <= bs::BlockShape3::kMaxH) return launch_block_shape<bs::BlockShape3>(p, wide != 0, d->num_sms, s);
+  return launch_block_shape<bs::BlockShape4>(p, wide != 0, d->num_sms, s);
 }
 
 }  // extern "C"
