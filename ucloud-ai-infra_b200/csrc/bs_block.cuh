@@ -11,7 +11,7 @@
 // Bound: HBM. Per token k (or 1) rows of bf16 and the residual are read, the residual and the e4m3 row written; what
 // costs is keeping enough of those reads in flight beside two reductions per row, in few instructions per element. A
 // producer warp brings the rows of the CTA's next tokens into a ring in shared memory by bulk copies, up to four rows
-// per stage, whatever the other warps are doing; two CTAs per SM, about 100 KB of ring each. The other warps own C
+// per stage, whatever the other warps are doing; the CTAs of an SM share about 200 KB of ring. The other warps own C
 // 16-byte chunks of a row each (chunk c = t + threads * j), add the ring's rows up as they land, and keep z and h in
 // registers between the two norms; a 128-group is the 16 chunks of a half-warp. Measured on the way (T = 8192,
 // H = 5120, k = 8): loads into registers by four CTAs of 320 threads 218 us; the ring with a stage per row 201 us, bound
@@ -26,6 +26,47 @@ constexpr int kBlockMaxH = 16384;
 
 enum : int { kGateNone = 0, kGateChannel = 1, kGateToken = 2, kGateFull = 3 };
 
+constexpr int kBlockMaxStages = 16;
+
+constexpr int kBlockResSlots = 2;
+
+// Shapes of the kernel: chunks per thread, most threads that own chunks (a producer warp comes on top), CTAs per SM that
+// its registers and its ring leave room for. By the row's length: some 20 warps per SM always, in as many CTAs as that
+// gives, since one CTA's reductions hide behind another's rows. Measured (T = 8192; us, dense and k = 8; H and two shapes):
+//   1024   <1, 128, 5> 25, 35   <2, 64, 8> 21, 32 (but 512: 15, 22 and 20, 26)   <1, 320, 2> 24, 51
+//   2048   <2, 160, 4> 38, 62   <1, 320, 2> 48, 67         2560   <2, 160, 4> 48, 77   <1, 320, 2> 56, 78
+//   8192   <2, 640, 1> 147, 221   <4, 320, 1> 179, 349
+template <int C_, int THREADS, int CTAS>
+struct BlockShape {
+  static constexpr int C = C_, kThreads = THREADS, kCtas = CTAS;
+  static constexpr int kMaxH = C * THREADS * 8;
+  static constexpr int kRingBytes = 200 * 1024 / CTAS;
+  static constexpr int kSums = (THREADS / 32 + 3) / 4 * 4;  // warp totals; those of warps that do not exist are 0
+  static_assert(kBlockResSlots * 4 * kMaxH + 2 * 2 * kMaxH <= kRingBytes, "fp32 residual rows and two stages");
+};
+using BlockShape1 = BlockShape<1, 128, 5>;
+using BlockShape2 = BlockShape<2, 160, 4>;
+using BlockShape3 = BlockShape<2, 320, 2>;
+using BlockShape4 = BlockShape<2, 640, 1>;
+using BlockShape5 = BlockShape<4, 512, 1>;
+static_assert(BlockShape5::kMaxH == kBlockMaxH, "every row has a shape");
+
+// The ring of a launch: two residual rows, and stages of G rows (a power of two), two at least.
+struct BlockRing {
+  int G, stages, res_bytes;  // res_bytes: a residual row's, 0 without one
+  int bytes(int H) const { return kBlockResSlots * res_bytes + stages * G * 2 * H; }
+};
+inline BlockRing block_ring(int k, int H, int res_bytes, int ring_bytes) {
+  BlockRing r = {k >= 3 ? 4 : k, 0, res_bytes};
+  const int room = ring_bytes - kBlockResSlots * res_bytes;
+  while (r.G > 1 && 2 * r.G * 2 * H > room) r.G >>= 1;
+  const int n = room / (r.G * 2 * H);
+  // Two stages of several rows keep enough reads in flight, and more of them cost (7168 x 8192 rows, k = 8: 200 us with
+  // two stages of four rows, 225 with three); of single rows 3, 6 and 16 are equal within 2 %.
+  const int most = r.G > 1 ? 2 : kBlockMaxStages;
+  r.stages = n < 2 ? 2 : n > most ? most : n;
+  return r;
+}
 struct BlockParams {
   const __nv_bfloat16* y;    // [rows_y, ldy]
   long long ldy;
@@ -48,44 +89,10 @@ struct BlockParams {
   float* As;                 // [T, H / 128]
   __nv_bfloat16* V;          // [T, H] or nullptr
   int T, H;
+  BlockRing ring;
   int* status;
 };
 
-constexpr int kBlockMaxStages = 16;
-
-constexpr int kBlockResSlots = 2;
-
-// Shapes of the kernel: chunks per thread, most threads that own chunks (a producer warp comes on top), CTAs per SM that
-// its registers and its ring leave room for. By the row's length: two small CTAs overlap one's reductions with the other's
-// reads; rows too long for them have one large CTA rather than more chunks a thread (T = 8192, k = 8, us; two chunks of
-// 640 threads against four chunks of 320: H = 6144 190 and 306, 8192 221 and 349).
-template <int C_, int THREADS, int CTAS>
-struct BlockShape {
-  static constexpr int C = C_, kThreads = THREADS, kCtas = CTAS;
-  static constexpr int kMaxH = C * THREADS * 8;
-  static constexpr int kRingBytes = 200 * 1024 / CTAS;
-  static constexpr int kSums = (THREADS / 32 + 3) / 4 * 4;  // warp totals; those of warps that do not exist are 0
-  static_assert(kBlockResSlots * 4 * kMaxH + 2 * 2 * kMaxH <= kRingBytes, "fp32 residual rows and two stages");
-};
-using BlockShape1 = BlockShape<1, 320, 2>;
-using BlockShape2 = BlockShape<2, 320, 2>;
-using BlockShape3 = BlockShape<2, 640, 1>;
-using BlockShape4 = BlockShape<4, 512, 1>;
-static_assert(BlockShape4::kMaxH == kBlockMaxH, "every row has a shape");
-
-// The ring of a launch: two residual rows, and stages of G rows (a power of two), two at least.
-struct BlockRing {
-  int G, stages, res_bytes;  // res_bytes: a residual row's, 0 without one
-  __host__ __device__ int bytes(int H) const { return kBlockResSlots * res_bytes + stages * G * 2 * H; }
-};
-__host__ __device__ inline BlockRing block_ring(int k, int H, int res_bytes, int ring_bytes) {
-  BlockRing r = {k >= 3 ? 4 : k, 0, res_bytes};
-  const int room = ring_bytes - kBlockResSlots * res_bytes;
-  while (r.G > 1 && 2 * r.G * 2 * H > room) r.G >>= 1;
-  const int n = room / (r.G * 2 * H);
-  r.stages = n < 2 ? 2 : n > kBlockMaxStages ? kBlockMaxStages : n;
-  return r;
-}
 // Sum over the `threads` consumer threads in a fixed order, in two halves so that other work can stand between them: a
 // butterfly per warp and its total in `buf`; then, after the barrier, every thread adds the warp totals. `buf` is not
 // reused before the next barrier.
@@ -133,8 +140,7 @@ __global__ void __launch_bounds__(Shape::kThreads + 32, Shape::kCtas) k_block_no
   const int t = threadIdx.x, nt = static_cast<int>(blockDim.x) - 32, lane = t & 31;
   const int nch = p.H / 8, row_bytes = 2 * p.H;
   const int k = p.weights ? p.k : 1;
-  const BlockRing br = block_ring(k, p.H, p.residual ? (WIDE ? 4 : 2) * p.H : 0, Shape::kRingBytes);
-  const int G = br.G, stages = br.stages, res_bytes = br.res_bytes;
+  const int G = p.ring.G, stages = p.ring.stages, res_bytes = p.ring.res_bytes;
   uint8_t* ring = block_smem + kBlockResSlots * res_bytes;
   for (int i = t; i < 4 * Shape::kSums; i += blockDim.x) (&sums[0][0][0])[i] = 0.f;
   if (t == 0) {
@@ -228,7 +234,8 @@ __global__ void __launch_bounds__(Shape::kThreads + 32, Shape::kCtas) k_block_no
 
   // -------------------------------------------------------------- rows
   // What every row uses, the norm weights' and a channel gate's chunks of this thread, is read again for each row (from
-  // L1), always ahead of a reduction: kept in registers it spills (8192 x 2560, one chunk a thread, k = 8: 83 us, 78 so).
+  // L1), always ahead of a reduction: kept in registers it spills (8192 x 2560, one chunk a thread,
+  // k = 8: 83 us, and 78 so).
   auto chunk = [&](const __nv_bfloat16* w, int c) {
     return w && c < nch ? __ldg(reinterpret_cast<const uint4*>(w + c * 8)) : make_uint4(0, 0, 0, 0);
   };

@@ -196,26 +196,28 @@ bs::GroupedParams grouped_params(const void* A, const float* As, const float* Bs
 }
 
 template <typename Shape, bool WIDE>
-int launch_block(const bs::BlockParams& p, int num_sms, cudaStream_t s) {
+int launch_block(bs::BlockParams& p, int num_sms, cudaStream_t s) {
   constexpr auto kern = bs::k_block_norm<Shape, WIDE>;
   const int res_bytes = p.residual ? (WIDE ? 4 : 2) * p.H : 0;
-  const int smem = bs::block_ring(p.weights ? p.k : 1, p.H, res_bytes, Shape::kRingBytes).bytes(p.H);
+  p.ring = bs::block_ring(p.weights ? p.k : 1, p.H, res_bytes, Shape::kRingBytes);
+  const int smem = p.ring.bytes(p.H);
   const int rc = prepare_kernel<kern>(Shape::kRingBytes, 0);
   if (rc != BS_OK) return rc;
   const int threads = ((p.H / 8 + Shape::C - 1) / Shape::C + 31) / 32 * 32;
-  int grid = p.T;  // a CTA per token, or as many as fit
+  int grid = p.T;  // a CTA per token, or as many as fit, with equal numbers of tokens
   if (p.T > num_sms) {
     int per_sm = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads + 32, smem) != cudaSuccess || per_sm < 1)
       per_sm = 1;
     cudaGetLastError();
-    grid = std::min(p.T, per_sm * num_sms);
+    const int rounds = (p.T - 1) / (per_sm * num_sms) + 1;
+    grid = (p.T - 1) / rounds + 1;
   }
   return launch_pdl(kern, grid, threads + 32, smem, s, "k_block_norm launch", p);
 }
 
 template <typename Shape>
-int launch_block_shape(const bs::BlockParams& p, bool wide, int num_sms, cudaStream_t s) {
+int launch_block_shape(bs::BlockParams& p, bool wide, int num_sms, cudaStream_t s) {
   return wide ? launch_block<Shape, true>(p, num_sms, s) : launch_block<Shape, false>(p, num_sms, s);
 }
 
@@ -349,7 +351,8 @@ int bs_fp8_block_norm_quant(const void* y, long long ldy, int rows_y, const floa
   if (H <= bs::BlockShape1::kMaxH) return launch_block_shape<bs::BlockShape1>(p, wide != 0, d->num_sms, s);
   if (H <= bs::BlockShape2::kMaxH) return launch_block_shape<bs::BlockShape2>(p, wide != 0, d->num_sms, s);
   if (H <= bs::BlockShape3::kMaxH) return launch_block_shape<bs::BlockShape3>(p, wide != 0, d->num_sms, s);
-  return launch_block_shape<bs::BlockShape4>(p, wide != 0, d->num_sms, s);
+  if (H <= bs::BlockShape4::kMaxH) return launch_block_shape<bs::BlockShape4>(p, wide != 0, d->num_sms, s);
+  return launch_block_shape<bs::BlockShape5>(p, wide != 0, d->num_sms, s);
 }
 
 }  // extern "C"
