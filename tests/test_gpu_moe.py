@@ -106,6 +106,29 @@ def test_dispatch(cuda_lib, T, k, E, begin, count):
     assert int(r.offsets.abs().max()) == 0 and bool((r.slot_row == -1).all()) and bool((r.row_token == -1).all())
 
 
+@pytest.mark.parametrize("T,E,k", [(29, 64, 9), (64, 16, 10), (200, 160, 32), (512, 40, 9), (513, 64, 9), (700, 512, 32),
+                                   (9500, 24, 5), (20000, 16, 8)])
+def test_plan_several_batches(cuda_lib, T, E, k):
+    """CTAs that rank their pairs in several batches: more than 256 pairs each, in one cluster (up to 512 tokens) and in two
+    launches. Few experts in a token's reach make long runs of one expert across batches; every call gives the same plan."""
+    g = torch.Generator().manual_seed(T + E + k)
+    logits = torch.randn(T, E, generator=g) + 2 * torch.randn(E, generator=g)
+    r = _ops().moe_route(logits.cuda(), k)
+    ids = torch.sort(logits, dim=1, descending=True, stable=True).indices[:, :k].to(torch.int32)
+    assert torch.equal(r.ids.cpu(), ids)
+    _check_plan(r, ids, 0, E)
+    begin, count = E // 4, E // 2
+    for _ in range(10):
+        _check_same(_ops().moe_route(logits.cuda(), k), r)
+        _check_same(_ops().moe_dispatch(r.ids, None, E), r)
+    _check_plan(_ops().moe_dispatch(r.ids, None, E, experts=(begin, count)), ids, begin, count)
+
+
+def _check_same(r, want):
+    for name in ("offsets", "row_token", "slot_row"):
+        assert torch.equal(getattr(r, name), getattr(want, name)), name
+
+
 # ----------------------------------------------------------------------------- grouped products
 def _case(counts, N, K, seed, spread=0):
     """Rows per expert -> (route tensors, weights and scales, tokens): every token in one slot, in shuffled order."""

@@ -156,7 +156,8 @@ __device__ __forceinline__ void route_scan(RouteSmem& sm, const RouteParams& p, 
 }
 
 // Ranks pairs [b, min(b + kRouteBatch, n1)) of this CTA by expert, in order, after those ranked before (sm.count, which
-// it brings up to date): slot_row gets the rank inside the CTA, -1 without a local expert.
+// it brings up to date): slot_row gets the rank inside the CTA, -1 without a local expert. A barrier has to stand between
+// two batches: the end of one reads the counts that the start of the next one zeroes.
 __device__ __forceinline__ void route_rank(RouteSmem& sm, const RouteParams& p, const int* ids, long long b, long long n1) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int nw = static_cast<int>(min(static_cast<long long>(kRouteBatch), n1 - b) + 31) / 32;
@@ -232,8 +233,10 @@ __global__ void __launch_bounds__(kRouteThreads) k_moe_route(const RouteParams p
   }
   const int* ids = VPL > 0 ? p.ids : p.ids_in;
   const long long n1 = static_cast<long long>(t1) * p.k;
-  for (long long b = static_cast<long long>(t0) * p.k; b < n1; b += kRouteBatch) route_rank(sm, p, ids, b, n1);
-  __syncthreads();
+  for (long long b = static_cast<long long>(t0) * p.k; b < n1; b += kRouteBatch) {
+    route_rank(sm, p, ids, b, n1);
+    __syncthreads();  // every warp has used this batch's counts
+  }
   if (p.hist) {
     if (tid < p.e_count) p.hist[static_cast<size_t>(blockIdx.x) * p.e_count + tid] = sm.count[tid];
     return;
