@@ -88,3 +88,53 @@ def test_host_tensors_are_refused():
         ops.moe_route(torch.zeros(4, 8), 2)
     with pytest.raises(ValueError):
         ops.block_norm_quant(torch.zeros(4, 128, dtype=torch.bfloat16), torch.zeros(4, 128, dtype=torch.bfloat16))
+
+
+# ----------------------------------------------------------------------------- weights at load
+def _expert_parameters(module, E=2, inter=128, H=256, device="cpu"):
+    for name, n, k in (("w13_weight", 2 * inter, H), ("w2_weight", H, inter)):
+        w = torch.arange(E * n * k, dtype=torch.int32).remainder(97).to(torch.uint8).view(torch.float8_e4m3fn).view(E, n, k)
+        setattr(module, name, torch.nn.Parameter(w.to(device), requires_grad=False))
+        scale = torch.ones(E, n // 128, k // 128)
+        setattr(module, name + "_scale_inv", torch.nn.Parameter(scale, requires_grad=False))
+    return module
+
+
+@pytest.fixture
+def hand(monkeypatch):
+    """The drop-in module as it runs on a B200, with the oracle's permute in place of the packing kernel."""
+    import fp8_hand_b200.fp8_hand_sm100 as hand
+    from oracle import oracle as O
+    monkeypatch.setattr(hand, "ENABLED", True)
+    monkeypatch.setattr(hand, "_is_b200", lambda: True)
+    monkeypatch.setattr(hand.ops, "pack_tiles", lambda w: O.relayout_tiles(w.view(torch.uint8)))
+    return hand
+
+
+def test_relayout_leaves_foreign_experts(hand):
+    """A module that has the parameter names but reads the row-major weights itself (SGLang's FusedMoE) keeps them."""
+    class FusedMoE(torch.nn.Module):
+        pass
+
+    moe = _expert_parameters(FusedMoE())
+    on_meta = _expert_parameters(FusedMoE(), device="meta")
+    kept = {k: v.clone() for k, v in moe.named_parameters()}
+    hand.relayout(torch.nn.ModuleList([moe, on_meta]))
+    for k, v in moe.named_parameters():
+        assert v.device.type == "cpu" and torch.equal(v.view(torch.uint8), kept[k].view(torch.uint8)), k
+    assert not any(hasattr(p, "tiles") for m in (moe, on_meta) for p in m.parameters())
+
+
+def test_relayout_moves_sparse_mlp(hand):
+    from fp8_hand_b200 import sglang_compat as S
+    src = _expert_parameters(torch.nn.Module())
+    mlp = S.SparseMLP(src.w13_weight.data, src.w13_weight_scale_inv.data, src.w2_weight.data, src.w2_weight_scale_inv.data, 1)
+    hand.relayout(torch.nn.Sequential(mlp))
+    assert mlp.w13_weight.device.type == mlp.w2_weight.device.type == "meta"
+    bytes13 = src.w13_weight.data.view(torch.uint8)
+    assert mlp.w13_weight.tiles.shape == (2, 2, 2, 128, 128)
+    assert torch.equal(mlp.w13_weight.tiles[1, 1, 0].view(torch.uint8), bytes13[1, 128:, :128])
+    assert hand.relayout_experts(mlp) == 0  # a second call finds nothing to do
+    del mlp.w13_weight.tiles
+    with pytest.raises(hand.tilepack.TilePackError, match="w13_weight: weight not loaded"):
+        hand.relayout(mlp)

@@ -8,7 +8,7 @@ import this module instead:
                                           SGLANG_FP8_HAND_FUSED_MIN_M (H:41-43)
   select(N, M) -> dict                    tile choice of an M x N product (H:74-81)
   precompile() -> list[str]               build step, never on the request path (H:596-611)
-  relayout(model, cache=None)             tile-first weight pre-pack after loading (H:652-672), expert weights included; with a
+  relayout(model, cache=None)             tile-first weight pre-pack after loading (H:652-672), SparseMLP's experts included; with a
                                           cache file (tilepack.py) the packed tiles are read, not permuted
   fused_gate_up(proj, x) -> (Q, Qs)|None  fused MLP front half (H:675-701)
   matmul(A, B, C, As, Bs, M, N, K, block_size) -> bool   GEMM hook (H:704-719)
@@ -142,10 +142,14 @@ EXPERT_WEIGHTS = ("w13_weight", "w2_weight")  # SGLang's FusedMoE parameter name
 
 
 def relayout_experts(model: torch.nn.Module) -> int:
-    """The expert weights of every mixture-of-experts module (e4m3 [E, N, K] with fp32 block scales [E, N/128, K/128]) to
-    tile-first storage [E, N/128, K/128, 128, 128]; returns how many were moved. Called by relayout."""
+    """The expert weights (e4m3 [E, N, K] with fp32 block scales [E, N/128, K/128]) of the modules that run on tiles to
+    tile-first storage [E, N/128, K/128, 128, 128]; returns how many were moved. Called by relayout. Such a module says so
+    by a true attribute `expert_tiles` (sglang_compat.SparseMLP does). Others keep their weights, SGLang's own FusedMoE
+    with the same parameter names above all: its kernels read the row-major storage."""
     moved = 0
-    for module in model.modules():
+    for path, module in model.named_modules():
+        if not getattr(module, "expert_tiles", False):
+            continue
         for name in EXPERT_WEIGHTS:
             weight, scale = getattr(module, name, None), getattr(module, name + "_scale_inv", None)
             if weight is None or scale is None or getattr(weight, "tiles", None) is not None:
@@ -155,6 +159,8 @@ def relayout_experts(model: torch.nn.Module) -> int:
             E, N, K = weight.shape
             if tuple(scale.shape) != (E, N // BK, K // BK):
                 continue
+            if weight.device.type == "meta":
+                raise tilepack.TilePackError(f"{path}.{name}: weight not loaded, and a tile cache holds no expert weights")
             tiles = ops.pack_tiles(weight.data.reshape(E * N, K)).view(E, N // BK, K // BK, BK, BK)
             setattr(module, name, Parameter(torch.empty(E, N, K, dtype=torch.float8_e4m3fn, device="meta"),
                                             requires_grad=False))

@@ -100,6 +100,8 @@ class SparseMLP(nn.Module):
     on the meta device and carry `.tiles`). E are the experts held here, numbers first_expert .. first_expert + E - 1
     of the router's (expert parallelism: the ranks' outputs add up)."""
 
+    expert_tiles = True  # relayout may move w13_weight and w2_weight
+
     def __init__(self, w13_weight: torch.Tensor, w13_weight_scale_inv: torch.Tensor, w2_weight: torch.Tensor,
                  w2_weight_scale_inv: torch.Tensor, top_k: int, *, renormalize: bool = True, routed_scale: float = 1.0,
                  first_expert: int = 0):
