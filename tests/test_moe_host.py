@@ -138,3 +138,18 @@ def test_relayout_moves_sparse_mlp(hand):
     del mlp.w13_weight.tiles
     with pytest.raises(hand.tilepack.TilePackError, match="w13_weight: weight not loaded"):
         hand.relayout(mlp)
+
+
+@pytest.mark.parametrize("experts,first,ok", [(4, 0, True), (2, 0, False), (2, 2, False), (4, 4, False), (6, 0, False)])
+def test_sparse_block_needs_every_expert(experts, first, ok):
+    """The norms are not linear: a block over some of the experts would normalise a partial sum."""
+    from fp8_hand_b200 import sglang_compat as S
+    src = _expert_parameters(torch.nn.Module(), E=experts)
+    mlp = S.SparseMLP(src.w13_weight.data, src.w13_weight_scale_inv.data, src.w2_weight.data, src.w2_weight_scale_inv.data, 1,
+                      first_expert=first)
+    norm, router = torch.ones(256, dtype=torch.bfloat16), torch.zeros(4, 256, dtype=torch.bfloat16)
+    if ok:
+        S.SparseBlock(router, mlp, norm)
+    else:
+        with pytest.raises(ValueError, match="every expert"):
+            S.SparseBlock(router, mlp, norm)

@@ -135,12 +135,16 @@ class SparseBlock(nn.Module):
     """A mixture-of-experts block between its norms. The stream between blocks is (h, A, As, v): the residual, the group
     quant of its norm (the experts' input) and the norm in bf16 (the router's). One call takes this block's
     (h, A, As, v) to the next's, whose norm weight is next_norm:
-      h' = residual_scale * h + scale * gate * rmsnorm(experts(A, As; router(v))) * post_norm"""
+      h' = residual_scale * h + scale * gate * rmsnorm(experts(A, As; router(v))) * post_norm
+    mlp holds every expert of the router: the norms need the sum over all of them, so a rank that holds some takes
+    SparseMLP.forward, adds the ranks' outputs, and ends the block with ops.block_norm_quant on the sum."""
 
     def __init__(self, router_weight: torch.Tensor, mlp: SparseMLP, next_norm: torch.Tensor,
                  post_norm: torch.Tensor | None = None, gate: torch.Tensor | None = None, scale: float = 1.0,
                  residual_scale: float = 1.0, eps: float = 1e-6):
         super().__init__()
+        if mlp.first_expert != 0 or mlp.w13_weight.shape[0] != router_weight.shape[0]:
+            raise ValueError("a block's mlp must hold every expert of its router")
         self.router_weight = nn.Parameter(router_weight, requires_grad=False)
         self.mlp = mlp
         self.next_norm = nn.Parameter(next_norm, requires_grad=False)
