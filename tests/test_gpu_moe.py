@@ -484,3 +484,26 @@ def test_refusals(cuda_lib):
         with pytest.raises(ValueError):
             ops.block_norm_quant(a.pop("y"), a.pop("residual"), **a)
     assert bool((y == 0).all())
+
+
+def test_refusals_of_too_few_rows(cuda_lib):
+    """A route for more tokens than there are rows: the products of the tokens that are not there, and their sums."""
+    ops = _ops()
+    bf, dev = torch.bfloat16, "cuda"
+    r = ops.moe_route(torch.zeros(5, 2, device=dev), 2)
+    A, As = ops.group_quant(torch.zeros(5, 256, dtype=bf, device=dev))
+    B, Bs = torch.zeros(2, 256, 256, dtype=torch.uint8, device=dev), torch.ones(2, 2, 2, device=dev)
+    y, res = torch.zeros(10, 256, dtype=bf, device=dev), torch.zeros(5, 256, dtype=bf, device=dev)
+    ops.grouped_gemm_silu_quant(A, B, As, Bs, r)
+    ops.grouped_gemm(A, B, As, Bs, r, gather=True)
+    ops.block_norm_quant(y, res, route=r)
+    with pytest.raises(ValueError, match="A has 4 rows, the route has 5 tokens"):
+        ops.grouped_gemm_silu_quant(A[:4], B, As[:4], Bs, r)
+    with pytest.raises(ValueError, match="A has 4 rows, the route has 5 tokens"):
+        ops.grouped_gemm(A[:4], B, As[:4], Bs, r, gather=True)
+    with pytest.raises(ValueError, match="A has 5 rows, the route has 10 rows"):
+        ops.grouped_gemm(A, B, As, Bs, r)
+    with pytest.raises(ValueError, match="y has 9 rows, the route has 10"):
+        ops.block_norm_quant(y[:9], res, route=r)
+    with pytest.raises(ValueError, match="y has 0 rows"):
+        ops.block_norm_quant(y[:0], None, route=r)

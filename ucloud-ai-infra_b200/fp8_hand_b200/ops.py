@@ -397,8 +397,9 @@ def grouped_gemm(A: torch.Tensor, B: torch.Tensor, As: torch.Tensor, Bs: torch.T
     expert e in `route`, bf16 or fp32 [T * k, N]. A holds the rows themselves (e.g. grouped_gemm_silu_quant's Q), or
     with gather=True the tokens. Rows past route.offsets[-1] are not written."""
     index, A, As, Bs, rows_a, R, hint, E, N, K = _check_grouped(A, B, As, Bs, route, b_tiled)
-    if not gather and rows_a < R:
-        raise ValueError(f"A has {rows_a} rows, the route has {R}")
+    need = route.slot_row.shape[0] if gather else R
+    if rows_a < need:
+        raise ValueError(f"A has {rows_a} rows, the route has {need} {'tokens' if gather else 'rows'}")
     if out is None:
         out, ldc = _matrix(R, N, out_dtype, A.device), N
     else:
@@ -420,6 +421,8 @@ def grouped_gemm_silu_quant(A: torch.Tensor, B: torch.Tensor, As: torch.Tensor, 
     in place through route.row_token. Returns Q e4m3 [T * k, I] and Qs fp32 [T * k, I/128] in row order; rows
     past route.offsets[-1] are not written."""
     index, A, As, Bs, rows_a, R, hint, E, N2, K = _check_grouped(A, B, As, Bs, route, b_tiled)
+    if rows_a < route.slot_row.shape[0]:
+        raise ValueError(f"A has {rows_a} rows, the route has {route.slot_row.shape[0]} tokens")
     if N2 % (2 * BLOCK):
         raise ValueError("gate_up rows must be a multiple of 256")
     dev = A.device
@@ -483,7 +486,7 @@ def block_norm_quant(y: torch.Tensor, residual: torch.Tensor | None, *, post_wei
       n = rmsnorm(z) * post_weight                     (post_weight None: n = z)
       h = residual_scale * residual + scale * gate * n
       A, As = group_quant(rmsnorm(h) * pre_weight)     (pre_weight None: not made)
-    y bf16 [T, H] (or [rows, H] with `route`), residual bf16 or fp32 [T, H] (None: h = scale * gate * n, bf16), gate
+    y bf16 [T, H] (or with `route` [T * k, H], or more rows), residual bf16 or fp32 [T, H] (None: h = scale * gate * n, bf16), gate
     bf16 [H], [T, 1] or [T, H]. h is rounded once, into `out` (a new tensor like residual; pass out=residual to update
     it in place); A is taken from the unrounded h. Returns (h, A e4m3 [T, H], As fp32 [T, H/128]), with norm_out also
     the norm itself in bf16 (a router's input), or h alone without pre_weight."""
@@ -534,6 +537,8 @@ def block_norm_quant(y: torch.Tensor, residual: torch.Tensor | None, *, post_wei
         w, rows = route.weights, route.slot_row
         if w is None or w.shape != rows.shape or rows.shape[0] != T:
             raise ValueError("the route must have weights, and a token for each row of the residual")
+        if rows_y < rows.numel():
+            raise ValueError(f"y has {rows_y} rows, the route has {rows.numel()}")
         if w.get_device() != index or rows.get_device() != index:
             _one_device(y, w, rows)
         if w.dtype != torch.float32 or rows.dtype != torch.int32 or not (w.is_contiguous() and rows.is_contiguous()):
