@@ -507,3 +507,21 @@ def test_refusals_of_too_few_rows(cuda_lib):
         ops.block_norm_quant(y[:9], res, route=r)
     with pytest.raises(ValueError, match="y has 0 rows"):
         ops.block_norm_quant(y[:0], None, route=r)
+
+
+def test_output_stride_beyond_32_bits(cuda_lib):
+    """Rows further apart than the C-ABI's 32-bit stride can say: refused, nothing written (the storage is 8.6 GB). A
+    stride just below is right, with the second row past 2^31 bytes."""
+    ops = _ops()
+    ids, B, Bs, A, As = _case([2], 256, 256, 3)
+    r = ops.moe_dispatch(ids.cuda(), None, 1)
+    off, src, _ = M.plan(ids, 0, 1)
+    dev = [t.cuda() for t in (A, B, As, Bs)]
+    out = torch.empty_strided((2, 256), ((1 << 32) + 256, 1), dtype=torch.bfloat16, device="cuda")
+    out.zero_()
+    with pytest.raises(ValueError, match="row stride"):
+        ops.grouped_gemm(*dev, r, gather=True, out=out)
+    assert bool((out == 0).all())
+    near = out.as_strided((2, 256), ((1 << 31) - 8, 1))
+    ops.grouped_gemm(*dev, r, gather=True, out=near)
+    _within(near, *M.grouped(A, As, B, Bs, off, src), BF16_HALF)

@@ -153,3 +153,13 @@ def test_sparse_block_needs_every_expert(experts, first, ok):
     else:
         with pytest.raises(ValueError, match="every expert"):
             S.SparseBlock(router, mlp, norm)
+
+
+@pytest.mark.parametrize("T,k", [((1 << 30) + 1, 1), (1 << 28, 5), (1 << 32, 1), ((1 << 32) + 4, 8)])
+def test_row_counts_beyond_32_bits_are_refused(T, k):
+    """Sizes that would wrap in the C-ABI's 32-bit arguments (2^32 tokens would be none)."""
+    from fp8_hand_b200 import ops
+    with pytest.raises(ValueError, match="rows"):
+        ops.moe_route(torch.zeros(1, 16).expand(T, 16), k)
+    with pytest.raises(ValueError, match="rows"):
+        ops.moe_dispatch(torch.zeros(1, k, dtype=torch.int32).expand(T, k), None, 16)

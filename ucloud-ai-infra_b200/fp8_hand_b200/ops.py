@@ -18,6 +18,7 @@ E4M3 = torch.float8_e4m3fn
 BLOCK = 128
 MAX_EXPERTS = 512
 MAX_TOP_K = 32
+MAX_ROWS = 1 << 30  # tokens times slots: rows are 32-bit on the device and in the C-ABI, which would wrap silently
 _BYTES = (E4M3, torch.uint8)
 
 
@@ -281,9 +282,10 @@ def _local_experts(experts, num_experts: int) -> tuple[int, int]:
     return begin, count
 
 
-def _routing_limits(num_experts: int, k: int) -> None:
+def _routing_limits(T: int, num_experts: int, k: int) -> None:
     _need(0 < num_experts <= MAX_EXPERTS, f"1 to {MAX_EXPERTS} experts are supported")
     _need(0 < k <= MAX_TOP_K, f"1 to {MAX_TOP_K} slots per token are supported")
+    _need(T * k <= MAX_ROWS, f"at most {MAX_ROWS} rows (tokens times slots) are supported")
 
 
 def _offsets_and_scratch(lib, T: int, count: int, device: torch.device):
@@ -304,11 +306,11 @@ def moe_route(logits: torch.Tensor, top_k: int, *, renormalize: bool = True, sca
     f32 = logits.dtype == torch.float32
     if logits.dim() != 2 or not (f32 or logits.dtype == torch.bfloat16):
         raise ValueError("logits must be bf16 or fp32 [T, E]")
-    index = _one_device(logits)
     T, E = logits.shape
-    if not (0 < E <= MAX_EXPERTS and 0 < top_k <= MAX_TOP_K and top_k <= E):
-        _routing_limits(E, top_k)
+    if not (0 < E <= MAX_EXPERTS and 0 < top_k <= MAX_TOP_K and top_k <= E and T * top_k <= MAX_ROWS):
+        _routing_limits(T, E, top_k)
         raise ValueError("top_k must be at most the number of experts")
+    index = _one_device(logits)
     begin, count = _local_experts(experts, E)
     ld, inner = logits.stride()
     if inner != 1 or ld < E:
@@ -332,6 +334,9 @@ def moe_dispatch(ids: torch.Tensor, weights: torch.Tensor | None, num_experts: i
     -1, has no row), weights fp32 [T, k] (None if no weighted sum follows)."""
     if ids.dim() != 2 or ids.dtype != torch.int32:
         raise ValueError("ids must be int32 [T, k]")
+    T, k = ids.shape
+    if not (0 < num_experts <= MAX_EXPERTS and 0 < k <= MAX_TOP_K and T * k <= MAX_ROWS):
+        _routing_limits(T, num_experts, k)
     if weights is not None:
         if weights.dtype != torch.float32 or weights.shape != ids.shape:
             raise ValueError("weights must be fp32 like ids")
@@ -339,8 +344,6 @@ def moe_dispatch(ids: torch.Tensor, weights: torch.Tensor | None, num_experts: i
         weights = weights.contiguous()
     else:
         index = _one_device(ids)
-    T, k = ids.shape
-    _routing_limits(num_experts, k)
     begin, count = _local_experts(experts, num_experts)
     ids = ids.contiguous()
     lib, dev = _native.lib(), ids.device
@@ -406,6 +409,8 @@ def grouped_gemm(A: torch.Tensor, B: torch.Tensor, As: torch.Tensor, Bs: torch.T
         if out.shape != (R, N) or out.get_device() != index or out.stride(1) != 1:
             raise ValueError("output must be [T * k, N] with contiguous rows, on the same device")
         ldc = out.stride(0) if R > 1 else N
+        if ldc >= 1 << 31:
+            raise ValueError("the output's row stride must be below 2^31 elements")
     f32 = out.dtype == torch.float32
     if not f32 and out.dtype != torch.bfloat16:
         raise ValueError("output must be bf16 or fp32")
