@@ -227,6 +227,36 @@ def test_grouped_several_slots(cuda_lib, T):
     assert torch.equal(Q.view(torch.uint8), Q2.view(torch.uint8)) and torch.equal(Qs, Qs2)
 
 
+@pytest.mark.parametrize("mean", [1, 10, 50])
+@pytest.mark.parametrize("bad", ["nan", "inf"])
+def test_silu_quant_not_finite(cuda_lib, mean, bad):
+    """A column that is NaN (an e4m3 NaN in a gate row of the weights) stays one NaN: its group's scale comes from the other
+    127 columns, in every kernel. Groups of infinite columns have an infinite scale."""
+    ops = _ops()
+    counts, inter = [60, 0, 7], 384  # by mean: token tiles of 16 and 32 rows, row tiles
+    ids, B, Bs, A, As = _case(counts, 2 * inter, 256, 19)
+    off, src, _ = M.plan(ids, 0, 3)
+    y, tol = M.silu_mul(*M.grouped(A, As, B, Bs, off, src))
+    cols = [5, 130, 131, 383]
+    if bad == "nan":
+        for c in cols:
+            B.view(torch.uint8)[0, c, 40] = 0x7F
+    else:
+        Bs = Bs.clone()
+        Bs[0, 0] = math.inf  # the gates of the first 128 columns: infinite, or NaN where an infinite sum has both signs
+    Q, Qs = ops.grouped_gemm_silu_quant(A.cuda(), B.cuda(), As.cuda(), Bs.cuda(), _route_for(ids, 3, mean))
+    Q, Qs, n = Q.cpu(), Qs.cpu(), counts[0]
+    if bad == "nan":
+        assert bool(Q.float()[:n, cols].isnan().all())
+        Q.view(torch.uint8)[:n, cols] = 0
+        y[:n, cols] = tol[:n, cols] = 0
+        M.check_quant(Q, Qs, y, tol, 1e-10 / 448)
+    else:
+        assert not bool(Q.float()[n:].isnan().any()) and not bool(Q.float()[:, 128:].isnan().any())
+        M.check_quant(Q[n:], Qs[n:], y[n:], tol[n:], 1e-10 / 448)
+        M.check_quant(Q[:n, 128:], Qs[:n, 1:], y[:n, 128:], tol[:n, 128:], 1e-10 / 448)
+
+
 # ----------------------------------------------------------------------------- the block's end
 def _block_case(T, H, k, wide, seed):
     g = torch.Generator().manual_seed(seed)

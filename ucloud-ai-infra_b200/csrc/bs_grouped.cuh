@@ -1003,7 +1003,8 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
         }
       } else {
         // y = silu(g) * u per (token, weight row), kept in this thread's own word of the gate partial; the group's
-        // amax is a warp maximum (|y| orders like its bits) and four warps' through shared memory.
+        // amax is a warp maximum (|y| orders like its bits) and four warps' through shared memory. A NaN counts as 0
+        // there, as in the row tiles (whose fmaxf drops it): it stays one NaN among well-scaled values.
         if (ok) {
           for (int j = wg; j < n_own; j += 2) {
             float g = 0.f, u = 0.f;
@@ -1013,7 +1014,7 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
             }
             const float y = silu_mul(g, u);
             xch[j * 128 + r] = y;
-            const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(y)));
+            const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(y), 0.f)));
             if (lane == 0) amx[j * 4 + q] = __uint_as_float(m);
           }
         }
