@@ -240,6 +240,15 @@ int bs_fp8_selftest_wait_timeout(uint64_t limit_ns, void* stream);
 #define BS_PLAN_FIELDS 14
 int bs_fp8_launch_plan(int M, int N, int K, int fused, int* plan, int n);
 
+/* How a grouped product runs on the current device (148 SMs assumed when no device is usable): the kernel and the tile that
+ * bs_fp8_grouped_gemm (fused = 0) or bs_fp8_grouped_gemm_silu_quant (1) choose for rows_hint expected rows (its R where the
+ * call gives no hint), E experts, N (N2) weight rows per expert and K. Fills plan[0 .. BS_GROUPED_FIELDS). */
+#define BS_GROUPED_KIND 0      /* 1 few rows per expert (the weights on the MMA's lanes), 2 row tiles */
+#define BS_GROUPED_TILE_ROWS 1 /* output rows of a tile                                               */
+#define BS_GROUPED_CLUSTER 2   /* CTAs that take a tile together, each a part of K                    */
+#define BS_GROUPED_FIELDS 3
+int bs_fp8_grouped_plan(int rows_hint, int E, int N, int K, int fused, int* plan, int n);
+
 /* Number of SMs the kernels size their persistent grids for (current device): all of them, or
  * BS_FP8_SM_LIMIT from the environment when that is smaller (SMs left to concurrent kernels). */
 int bs_fp8_num_sms(void);

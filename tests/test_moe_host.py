@@ -58,6 +58,38 @@ def test_grouped_arguments(lib):
         assert lib.bs_fp8_grouped_gemm_silu_quant(*{**fused, **bad}.values(), None) == 1, bad
 
 
+# rows expected, experts, N (N2), K, fused -> kind, rows per tile, CTAs per tile, on 148 SMs (or as many as are there)
+GROUPED_PLANS = [
+    ((8, 64, 2048, 5120, True), (1, 16, 2)),      # one token: 64 tiles
+    ((488, 64, 2048, 5120, True), (1, 32, 2)),    # more tiles than SMs, fused: two CTAs per tile
+    ((488, 64, 5120, 1024, False), (1, 32, 1)),   # plain: one
+    ((1025, 64, 2048, 5120, True), (2, 128, 1)),  # more than 16 rows per expert
+    ((897, 64, 5120, 1024, False), (2, 128, 1)),  # more than 14
+    ((4, 1, 256, 1920, False), (1, 16, 1)),       # fewer than 16 K blocks
+    ((4, 1, 256, 2048, False), (1, 16, 2)),
+    ((5, 1, 256, 4096, False), (1, 32, 4)),
+    ((5, 1, 512, 8192, True), (1, 32, 8)),
+    ((5, 1, 512, 65536, True), (1, 32, 8)),
+]
+
+
+@pytest.mark.parametrize("shape,want", GROUPED_PLANS)
+def test_grouped_plan(lib, shape, want):
+    from fp8_hand_b200 import _native
+    if _native.num_sms() not in (0, 148):
+        pytest.skip("the rule goes by the number of SMs")
+    assert tuple(_native.grouped_plan(*shape).values()) == want
+
+
+def test_grouped_plan_arguments(lib):
+    from fp8_hand_b200 import _native
+    for bad in ((0, 1, 256, 256, False), (4, 0, 256, 256, False), (4, 513, 256, 256, False), (4, 1, 200, 256, False),
+                (4, 1, 384, 256, True), (4, 1, 256, 200, False)):
+        with pytest.raises(RuntimeError):
+            _native.grouped_plan(*bad)
+    assert lib.bs_fp8_grouped_plan(4, 1, 256, 256, 0, None, 3) == 1
+
+
 def test_block_arguments(lib):
     ok = dict(y=P, ldy=256, rows=4, w=None, sr=None, k=0, res=P, ldr=256, out=P, ldo=256, wide=0, post=None, gate=None, kind=0,
               ldg=0, scale=1.0, rscale=1.0, pre=P, eps=1e-6, A=P, As=P, V=None, T=4, H=256)

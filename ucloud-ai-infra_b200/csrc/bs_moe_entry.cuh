@@ -302,6 +302,18 @@ int bs_fp8_grouped_gemm_silu_quant(const void* A, const void* B, void* Q, const 
   return run_grouped<true>(A, B, p, rows_hint ? rows_hint : R, static_cast<cudaStream_t>(stream), d->num_sms);
 }
 
+int bs_fp8_grouped_plan(int rows_hint, int E, int N, int K, int fused, int* plan, int n) {
+  if (!plan || n < BS_GROUPED_FIELDS) return BS_ERR_ARG;
+  if (rows_hint <= 0 || E <= 0 || E > bs::kMaxExperts || N <= 0 || N % (fused ? 256 : 128) || K <= 0 || K % 128) return BS_ERR_ARG;
+  DeviceState* d = device_state();
+  const GroupedPlan g = grouped_plan(fused != 0, E, N / 128, K / 128, rows_hint, d ? d->num_sms : 148);
+  for (int i = 0; i < n; ++i) plan[i] = 0;
+  plan[BS_GROUPED_KIND] = g.nt ? 1 : 2;
+  plan[BS_GROUPED_TILE_ROWS] = g.nt ? g.nt : 128;
+  plan[BS_GROUPED_CLUSTER] = 1 << g.log_s;
+  return BS_OK;
+}
+
 int bs_fp8_block_norm_quant(const void* y, long long ldy, int rows_y, const float* weights, const int* slot_row,
                             int top_k, const void* residual, long long ldr, void* out, long long ldo, int wide,
                             const void* post_weight, const void* gate, int gate_kind, long long ldg, float scale,

@@ -48,6 +48,7 @@ SIGNATURES = {
     "bs_fp8_status": (_I, [ctypes.POINTER(_I), _I]),
     "bs_fp8_selftest_wait_timeout": (_I, [_U64, _VP]),
     "bs_fp8_launch_plan": (_I, [_I, _I, _I, _I, ctypes.POINTER(_I), _I]),
+    "bs_fp8_grouped_plan": (_I, [_I, _I, _I, _I, _I, ctypes.POINTER(_I), _I]),
     "bs_fp8_num_sms": (_I, []),
     "bs_fp8_error_string": (ctypes.c_char_p, [_I]),
     "bs_fp8_abi_version": (_I, []),
@@ -170,6 +171,17 @@ def launch_plan(M: int, N: int, K: int, fused: bool) -> dict:
     check(lib().bs_fp8_launch_plan(int(M), int(N), int(K), int(bool(fused)), buf, len(PLAN_FIELDS)),
           "bs_fp8_launch_plan")
     return dict(zip(PLAN_FIELDS, list(buf)))
+
+
+GROUPED_FIELDS = ("kind", "tile_rows", "cluster")  # include/bs_fp8.h BS_GROUPED_*
+
+
+def grouped_plan(rows: int, E: int, N: int, K: int, fused: bool) -> dict:
+    """How a product grouped by expert runs for `rows` expected rows (ops.grouped_gemm, fused: grouped_gemm_silu_quant)."""
+    buf = (ctypes.c_int * len(GROUPED_FIELDS))()
+    check(lib().bs_fp8_grouped_plan(int(rows), int(E), int(N), int(K), int(bool(fused)), buf, len(GROUPED_FIELDS)),
+          "bs_fp8_grouped_plan")
+    return dict(zip(GROUPED_FIELDS, list(buf)))
 
 
 def num_sms() -> int:
