@@ -227,6 +227,89 @@ def test_grouped_several_slots(cuda_lib, T):
     assert torch.equal(Q.view(torch.uint8), Q2.view(torch.uint8)) and torch.equal(Qs, Qs2)
 
 
+SPLIT_COUNTS = {"few": [3, 0, 1, 16, 17, 0, 2], "many": [100, 0, 300, 3]}
+
+
+def _plan_is(rows, E, N, K, fused, want):
+    from fp8_hand_b200 import _native
+    assert _native.num_sms() == 148, "the clusters below are chosen for 148 SMs"
+    p = _native.grouped_plan(rows, E, N, K, fused)
+    assert (p["kind"], p["tile_rows"], p["cluster"]) == (1, *want), p
+
+
+@pytest.mark.parametrize("fused", [False, True])
+@pytest.mark.parametrize("counts", sorted(SPLIT_COUNTS))
+@pytest.mark.parametrize("tile", [16, 32])
+@pytest.mark.parametrize("K,cluster", [(2048, 2), (2176, 2), (4096, 4), (5248, 4), (8192, 8), (8320, 8)])
+def test_grouped_clusters(cuda_lib, fused, counts, tile, K, cluster):
+    """Tiles whose K is split over 2, 4 and 8 CTAs, evenly and not: tiles with fewer rows than CTAs (some finish no row), and
+    more tiles than clusters, so that each uses its exchange buffer several times. Every run gives the same bits."""
+    ops = _ops()
+    c = SPLIT_COUNTS[counts]
+    E, N = len(c), 512 if fused else 256
+    ids, B, Bs, A, As = _case(c, N, K, 23)
+    R = ids.numel()
+    rows = {16: E, 32: 5 * E}[tile]                    # rows that the call expects, by the experts in all
+    experts = R * E // rows if counts == "many" else {16: R, 32: E}[tile]
+    rows = min(R, -(-R * E // experts))
+    _plan_is(rows, E, N, K, fused, (tile, cluster))
+    r = ops.moe_dispatch(ids.cuda(), None, E)
+    r.num_experts = experts
+    off, src, _ = M.plan(ids, 0, E)
+    ref, tol = M.grouped(A, As, B, Bs, off, src)
+    dev = [t.cuda() for t in (A, B, As, Bs)]
+    if fused:
+        y, ty = M.silu_mul(ref, tol)
+        Q, Qs = ops.grouped_gemm_silu_quant(*dev, r)
+        M.check_quant(Q.cpu(), Qs.cpu(), y, ty, 1e-10 / 448)
+        for _ in range(5):
+            Q2, Qs2 = ops.grouped_gemm_silu_quant(*dev, r)
+            assert torch.equal(Q.view(torch.uint8), Q2.view(torch.uint8)) and torch.equal(Qs, Qs2)
+    else:
+        out = ops.grouped_gemm(*dev, r, gather=True, out_dtype=torch.float32)
+        _within(out, ref, tol)
+        order = src.long()
+        rows_in_order = A.view(torch.uint8)[order].view(torch.float8_e4m3fn).cuda()
+        tiles = _tiles(B)
+        for _ in range(5):
+            assert torch.equal(ops.grouped_gemm(*dev, r, gather=True, out_dtype=torch.float32), out)
+            got = ops.grouped_gemm(rows_in_order, tiles, As[order].cuda(), dev[3], r, b_tiled=True)
+            assert torch.equal(got, out.to(torch.bfloat16))
+    from fp8_hand_b200 import _native
+    assert _native.status() == 0
+
+
+@pytest.mark.parametrize("tile", [16, 32])
+def test_grouped_clusters_more_tiles_than_sms(cuda_lib, tile):
+    """The fused product on two CTAs per tile with more tiles than SMs: every cluster walks several tiles."""
+    ops = _ops()
+    E, N, K = 38, 1024, 2048
+    c = [1 + e % 3 for e in range(E)]
+    c[5], c[20] = 40, 17
+    ids, B, Bs, A, As = _case(c, N, K, 29)
+    R = ids.numel()
+    assert E < R <= 4 * E
+    _plan_is(R, E, N, K, True, (16, 2))
+    r = ops.moe_dispatch(ids.cuda(), None, E)
+    if tile == 32:  # the same rows, and slots of no expert
+        spread = 4 * E + 1 - R
+        ids = torch.cat([ids, torch.full((spread, 1), -1, dtype=torch.int32)])
+        A = torch.cat([A.view(torch.uint8), torch.zeros(spread, K, dtype=torch.uint8)]).view(torch.float8_e4m3fn)
+        As = torch.cat([As, torch.ones(spread, K // 128)])
+        _plan_is(ids.numel(), E, N, K, True, (32, 2))
+        r = ops.moe_dispatch(ids.cuda(), None, E)
+    off, src, _ = M.plan(ids, 0, E)
+    y, tol = M.silu_mul(*M.grouped(A, As, B, Bs, off, src))
+    dev = [t.cuda() for t in (A, _tiles(B), As, Bs)]
+    Q, Qs = ops.grouped_gemm_silu_quant(*dev, r, b_tiled=True)
+    M.check_quant(Q[:R].cpu(), Qs[:R].cpu(), y, tol, 1e-10 / 448)
+    for _ in range(10):
+        Q2, Qs2 = ops.grouped_gemm_silu_quant(*dev, r, b_tiled=True)
+        assert torch.equal(Q[:R].view(torch.uint8), Q2[:R].view(torch.uint8)) and torch.equal(Qs[:R], Qs2[:R])
+    from fp8_hand_b200 import _native
+    assert _native.status() == 0
+
+
 @pytest.mark.parametrize("mean", [1, 10, 50])
 @pytest.mark.parametrize("bad", ["nan", "inf"])
 def test_silu_quant_not_finite(cuda_lib, mean, bad):

@@ -15,7 +15,7 @@
 //                     5120 -> 2 x 1024 858 us, plain 1024 -> 5120 475 us (1.5 PFLOP/s, at 1.45-1.65 GHz under the
 //                     1000 W limit; a tile costs 128 rows whatever it holds)
 //   k_grouped_tokens  128 weight rows on the lanes, up to 16 or 32 rows on the columns, for experts with few rows. Bound by
-//                     the weights' stream: 61 tokens x 8 of 64 experts, the same products: 101 us (6.65 TB/s), 58 us;
+//                     the weights' stream: 61 tokens x 8 of 64 experts, the same products: 100 us (6.7 TB/s), 58 us;
 //                     one token: 18.5 us for 84 MB, of which some 6 us are the start (the plan, the first boxes) and end
 #pragma once
 #include "bs_common.cuh"
@@ -583,7 +583,8 @@ __global__ void __launch_bounds__(GroupedRowsCfg<FUSED, BOX>::kThreads, 1)
 // through global memory.
 //
 // CTA layout (384 threads): warps 0-7 promotion (warpgroup g: tokens [g * NT/2, ...)) and epilogue, warp 8 TMA
-// producer, warp 9 TMEM + MMA issuer, warps 10-11 scale products As[src, kb] * Bs[nb, kb] into a ring of eight slots.
+// producer, warp 9 TMEM + MMA issuer, warp 10 scale products As[src, kb] * Bs[nb, kb] into a ring of eight slots, warp 11
+// hands the exchange buffer back to the cluster.
 // A unit of the pipeline is kKu K blocks of a tile (32 KB of weights): gate and up of one K block, or two K blocks of
 // one weight block, each set of partials in TMEM columns of its own.
 template <bool FUSED, int NT>
@@ -593,6 +594,7 @@ struct GroupedTokensCfg {
   static constexpr int kKu = FUSED ? 1 : 2;
   static constexpr int kSets = kNwg * kKu;
   static constexpr int kTr = NT / 2;
+  static_assert(NT <= 32, "a lane of the scale warp per token");
   static constexpr int kWBytes = 16384 * kNwg;  // per K block
   static constexpr int kXBytes = NT * 128;
   static constexpr int kBlockBytes = kWBytes + ((kXBytes + 1023) / 1024) * 1024;
@@ -638,6 +640,10 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t pa
       : "memory");
   return ok != 0;
 }
+// Remote arrival that releases what the thread has read and written, and what it has acquired, to the cluster.
+__device__ __forceinline__ void mbar_arrive_remote_release(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 // mbar_wait_warp that also acquires what CTAs of the cluster published.
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort, int* status) {
   if (__all_sync(0xffffffffu, mbar_try_wait_cluster(bar, parity))) return true;
@@ -679,9 +685,10 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
   uint64_t* drain = sempty + NS;
   uint64_t* rfull = drain + 1;   // every CTA's partials of this CTA's tokens are here
   uint64_t* rempty = rfull + 1;  // every CTA has read the partials of the previous tile
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rempty + 1);
+  uint64_t* rread = rempty + 1;  // this CTA's warps have
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rread + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((2 * ST + 2 * NB + 2 * NS + 3) * 8 + 8 <= Cfg::kBarBytes, "barrier area");
+  static_assert((2 * ST + 2 * NB + 2 * NS + 4) * 8 + 8 <= Cfg::kBarBytes, "barrier area");
   GroupTable& table = *reinterpret_cast<GroupTable*>(smem + Cfg::kTableOff);
 
   const int warp = threadIdx.x >> 5;
@@ -698,12 +705,13 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
       mbar_init(&pempty[i], 256);
     }
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&sfull[i], 64);
+      mbar_init(&sfull[i], 32);
       mbar_init(&sempty[i], 256);
     }
     mbar_init(drain, 1);
     mbar_init(rfull, 1);
-    mbar_init(rempty, 8 * S);
+    mbar_init(rempty, S);
+    mbar_init(rread, 8);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmW);
@@ -827,30 +835,35 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
       mma_commit(drain);
       mbar_wait(drain, 0, abort_flag, p.status, kErrTimeoutDrain, 100000000ull);
     }
-  } else if (warp >= 10) {
+  } else if (warp == 11) {
+    // ------------------------------------------------------------ the exchange buffer, back to the cluster
+    // What the promotion warps have read and written there is behind this CTA's barrier, and the arrivals release it to
+    // the CTAs that write the next partials. A warp of its own, since a release to the cluster takes its time and the
+    // next tile needs it only at its end: with the promotion warps releasing, 61 tokens take 103.5 us instead of 100.0,
+    // 128 experts and 160 tokens 79.5 instead of 67.4.
+    if (log_s > 0) {
+      uint32_t ph = 0;
+      for (int tile = first; tile < num_tiles; tile += step, ph ^= 1) {
+        if (!mbar_wait_warp(rread, ph, abort_flag, p.status, kErrTimeoutCluster)) break;
+        if (lane < S) mbar_arrive_remote_release(mapa_shared(rempty, lane));
+      }
+    }
+  } else if (warp == 10) {
     // ------------------------------------------------------------ scale products
-    constexpr int TPL = (NT + 63) / 64;
-    const int tok_base = (warp - 10) * 32 * TPL + lane;
     int slot = 0;
     uint32_t sph = 0;
     bool ok = true;
     for (int tile = first; ok && tile < num_tiles; tile += step) {
       const GroupTile t = find_tile(table, tile, NT);
-      const float* arow[TPL];
-#pragma unroll
-      for (int j = 0; j < TPL; ++j) {
-        const int tok = tok_base + 32 * j;
-        arow[j] = p.As + static_cast<size_t>(source_row(p, t.row + (tok < t.rows ? tok : 0))) * KB;
-      }
+      const float* arow = p.As + static_cast<size_t>(source_row(p, t.row + (lane < t.rows ? lane : 0))) * KB;
       const float* brow = p.Bs + (static_cast<size_t>(t.expert) * nblk + t.tn) * KB;
       const float* urow = brow + static_cast<size_t>(I_blk) * KB;
-      float a[2][KU][TPL], bw[2][KU][NWG];  // operands of this unit and the next
+      float a[2][KU], bw[2][KU][NWG];  // operands of this unit and the next
       auto load = [&](int u, int kb) {
 #pragma unroll
         for (int h = 0; h < KU; ++h) {
           const int k = min(kb + h, kb1 - 1);
-#pragma unroll
-          for (int j = 0; j < TPL; ++j) a[u][h][j] = ldg_f32(arow[j] + k);
+          a[u][h] = ldg_f32(arow + k);
 #pragma unroll
           for (int w = 0; w < NWG; ++w) bw[u][h][w] = ldg_f32((w == 0 ? brow : urow) + k);
         }
@@ -861,15 +874,12 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
           return;
         }
         float* dst = ring + slot * (NSET * NT);
+        if (lane < NT) {
 #pragma unroll
-        for (int h = 0; h < KU; ++h)
+          for (int h = 0; h < KU; ++h)
 #pragma unroll
-          for (int w = 0; w < NWG; ++w)
-#pragma unroll
-            for (int j = 0; j < TPL; ++j) {
-              const int tok = tok_base + 32 * j;
-              if (tok < NT) dst[(h * NWG + w) * NT + tok] = tok < t.rows ? __fmul_rn(a[u][h][j], bw[u][h][w]) : 0.f;
-            }
+            for (int w = 0; w < NWG; ++w) dst[(h * NWG + w) * NT + lane] = lane < t.rows ? __fmul_rn(a[u][h], bw[u][h][w]) : 0.f;
+        }
         mbar_arrive(&sfull[slot]);
         load(u, kb_next);
         if (++slot == NS) {
@@ -967,7 +977,7 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
       } else if (ok) {
         // The owner's barrier counts the bytes, so no fence stands between the words and their reader.
         if (threadIdx.x == 0) mbar_arrive_expect_tx(rfull, n_own * S * NWG * 512);
-        ok = mbar_wait_warp(rempty, rph ^ 1, abort_flag, p.status, kErrTimeoutCluster);
+        ok = mbar_wait_cluster(rempty, rph ^ 1, abort_flag, p.status);
         if (ok) {
 #pragma unroll
           for (int i = 0; i < TR; ++i) {
@@ -1035,11 +1045,8 @@ __global__ void __launch_bounds__(GroupedTokensCfg<FUSED, NT>::kThreads, 1)
         }
       }
       if (ok && log_s > 0) {
-        // This warp's reads are done: each value read went into a store above, so no load is still under way when the
-        // arrival issues, and the count alone is enough. (A releasing arrival also waits for those stores to reach
-        // global memory: 61 tokens 101.0 -> 104.2 us, 128 experts and 160 tokens 67.5 -> 78.2.)
         __syncwarp();
-        if (lane < S) mbar_arrive_remote_relaxed(mapa_shared(rempty, lane));
+        if (lane == 0) mbar_arrive(rread);
       }
       rph ^= 1;
     }
