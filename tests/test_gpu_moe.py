@@ -404,6 +404,25 @@ def test_block_row_lengths(cuda_lib, T, H, k, wide):
     _check_block(got, M.block(y, res, post=post, gate=gt, pre=pre, weights=w, slot_row=slot, **kw), wide)
 
 
+@pytest.mark.parametrize("T,H", [(14300, 128), (2300, 1024), (2300, 1152), (2300, 2560), (1350, 2688), (1000, 5120),
+                                 (460, 5248), (460, 10240), (460, 10368), (460, 16384)])
+@pytest.mark.parametrize("k,wide", [(0, False), (6, False), (5, True)])
+def test_block_many_rows_per_cta(cuda_lib, T, H, k, wide):
+    """The first and the last length of each of the kernel's shapes with at least three rows per CTA: the ring's stages, both
+    residual slots and both sets of sums are used again."""
+    y, res, post, pre, w, slot, g = _block_case(T, H, k, wide, T + H + k)
+    gt = torch.sigmoid(torch.randn(T, 1, generator=g)).to(torch.bfloat16)
+    kw = dict(scale=0.8, residual_scale=0.9, eps=1e-6)
+    dev = (y.cuda(), res.cuda())
+    more = dict(post_weight=post.cuda(), gate=gt.cuda(), pre_weight=pre.cuda(), route=_route_of(w, slot), **kw)
+    got = _ops().block_norm_quant(*dev, **more)
+    _check_block(got, M.block(y, res, post=post, gate=gt, pre=pre, weights=w, slot_row=slot, **kw), wide)
+    again = _ops().block_norm_quant(*dev, **more)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, again))
+    from fp8_hand_b200 import _native
+    assert _native.status() == 0
+
+
 @pytest.mark.parametrize("H", [640, 5120, 8192])
 def test_block_scales_at_their_floor(cuda_lib, H):
     """Groups whose norm weight is so small that the scale is at its floor beside ordinary ones."""

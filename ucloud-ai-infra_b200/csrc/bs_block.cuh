@@ -119,7 +119,6 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
       : "memory");
 }
 
-// blockDim = threads that own chunks + the producer warp.
 // amax / 448, correctly rounded by one correction step (bs_quant.cuh, group_scale), without its floor.
 __device__ __forceinline__ float amax_div_448(float amax) {
   constexpr float kInv448 = 1.0f / 448.0f;
@@ -127,6 +126,7 @@ __device__ __forceinline__ float amax_div_448(float amax) {
   return __fmaf_rn(__fmaf_rn(-448.0f, q0, amax), kInv448, q0);
 }
 
+// blockDim = threads that own chunks + the producer warp.
 template <typename Shape, bool WIDE>
 __global__ void __launch_bounds__(Shape::kThreads + 32, Shape::kCtas) k_block_norm(const BlockParams p) {
   constexpr int C = Shape::C;
@@ -205,6 +205,7 @@ __global__ void __launch_bounds__(Shape::kThreads + 32, Shape::kCtas) k_block_no
       for (int s = 0; s < k; s += G) {
         if (lane == 0) ok = mbar_wait(&empty[st], ph ^ 1, &abort_flag, p.status, kErrTimeoutEmpty);
         ok = __shfl_sync(0xffffffffu, ok, 0);
+        __syncwarp();  // the other lanes too come after the readers of this stage: the shuffle orders no memory
         if (!ok) break;
         // lanes s .. s + G - 1 bring their slots' rows (lanes from k on have none)
         const uint32_t mask = (has >> s) & ((1u << G) - 1);
