@@ -178,8 +178,8 @@ size_t bs_fp8_moe_scratch_bytes(int T, int e_count);
 
 /* Products grouped by expert. Weights: E experts of bs_fp8_gemm's formats one after another (row-major [E, N, K] or
  * tile-first [E, N/128, K/128, 128, 128]), Bs [E, N/128, K/128]. Row r of the output, offsets[e] <= r < offsets[e + 1],
- * is row row_token[r] of A (row r where row_token is NULL) times expert e's weights; rows past offsets[E] are
- * not written. A [rows_a, K], As [rows_a, K/128]; R rows of output. rows_hint: rows that the caller expects
+ * is row row_token[r] of A (row r where row_token is NULL; row 0 for a token outside [0, rows_a)) times expert e's weights;
+ * rows past offsets[E] are not written. A [rows_a, K], As [rows_a, K/128]; R rows of output. rows_hint: rows that the caller expects
  * in all (at most R; 0: R); it only chooses between kernels. E <= 512.
  *   bs_fp8_grouped_gemm             C [R, ldc] bf16 (out_dtype 0) or fp32 (1), as bs_fp8_gemm
  *   bs_fp8_grouped_gemm_silu_quant  Q [R, I], Qs [R, I/128] with N2 = 2 * I gate and up rows per expert, as

@@ -35,7 +35,9 @@ constexpr int kBlockResSlots = 2;
 // gives, since one CTA's reductions hide behind another's rows. Measured (T = 8192; us, dense and k = 8; H and two shapes):
 //   1024   <1, 128, 5> 25, 35   <2, 64, 8> 21, 32 (but 512: 15, 22 and 20, 26)   <1, 320, 2> 24, 51
 //   2048   <2, 160, 4> 38, 62   <1, 320, 2> 48, 67         2560   <2, 160, 4> 48, 77   <1, 320, 2> 56, 78
-//   8192   <2, 640, 1> 147, 221   <4, 320, 1> 179, 349
+//   8192   <2, 640, 1> 147, 221   <4, 320, 1> 179, 349     12288  <4, 512, 1> 295, 466     16384  <4, 512, 1> 323, 575
+// Spills: <4, 512, 1> 52 bytes (92 with an fp32 residual), the others none (8 to 16 with an fp32 residual and C = 2).
+// With an fp32 residual: 2048 45, 71; 5120 105, 190; 16384 376, 749.
 template <int C_, int THREADS, int CTAS>
 struct BlockShape {
   static constexpr int C = C_, kThreads = THREADS, kCtas = CTAS;

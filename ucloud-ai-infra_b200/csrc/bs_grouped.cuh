@@ -13,10 +13,11 @@
 //   k_grouped_rows    128 rows x 256 weight columns per tile, rows on the MMA's 128 lanes, for experts with many rows. Bound
 //                     by the promotion of each K block's partial and by power: 8192 tokens x 8 of 64 experts, fused
 //                     5120 -> 2 x 1024 858 us, plain 1024 -> 5120 475 us (1.5 PFLOP/s, at 1.45-1.65 GHz under the
-//                     1000 W limit; a tile costs 128 rows whatever it holds)
+//                     1000 W limit; a tile costs 128 rows whatever it holds). The plain product with fp32 output, whose
+//                     threads write 16 bytes of a row each, takes 1086 us. The fused form spills 8 bytes (68 reloaded).
 //   k_grouped_tokens  128 weight rows on the lanes, up to 16 or 32 rows on the columns, for experts with few rows. Bound by
 //                     the weights' stream: 61 tokens x 8 of 64 experts, the same products: 100 us (6.7 TB/s), 58 us;
-//                     one token: 18.5 us for 84 MB, of which some 6 us are the start (the plan, the first boxes) and end
+//                     one token: 18.7 us for 84 MB, of which some 6 us are the start (the plan, the first boxes) and end
 #pragma once
 #include "bs_common.cuh"
 #include "bs_prefill.cuh"
